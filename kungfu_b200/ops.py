@@ -1404,5 +1404,147 @@ def topk_lse(logits, k: int, out_ids, out_vals, out_lse) -> None:
     add_launches(1)
 
 
+# ---- log probabilities and copies of pages ----------------------------------------------------------------------------
+
+def _same_device(what: str, *tensors) -> None:
+    """Every tensor of a call lives on one device, and that is the one launches go to."""
+    devices = {t.device for t in tensors if t is not None}
+    if len(devices) > 1:
+        raise KernelError(f"{what}: tensors on several devices ({', '.join(sorted(str(d) for d in devices))})")
+    for d in devices:
+        if d.type == "cuda" and d.index != torch.cuda.current_device():
+            raise KernelError(f"{what}: tensors on {d}, but the current device is cuda:{torch.cuda.current_device()}")
+
+
+def _check_out(what: str, name: str, t, shape: tuple, dtype: torch.dtype) -> None:
+    if t is not None and (tuple(t.shape) != shape or t.dtype != dtype or not t.is_contiguous()):
+        raise KernelError(f"{what}: {name} is {tuple(t.shape)} {t.dtype}, not contiguous {shape} {dtype}")
+
+
+def _check_tokens(what: str, tokens, rows: int, logprob, rank=None) -> None:
+    if tokens is None:
+        if logprob is not None or rank is not None:
+            raise KernelError(f"{what}: log probabilities and ranks need the tokens they are of")
+        return
+    if tuple(tokens.shape) != (rows,) or tokens.dtype != torch.int32 or not tokens.is_contiguous():
+        raise KernelError(f"{what}: tokens are {tuple(tokens.shape)} {tokens.dtype}, not contiguous ({rows},) torch.int32")
+    _check_out(what, "out_logprob", logprob, (rows,), torch.float32)
+    _check_out(what, "out_rank", rank, (rows,), torch.int32)
+
+
+MAX_TOP_LOGPROBS = 64           # alternatives that `token_logprobs` ranks
+
+
+@_dispatch("token_logprobs")
+def token_logprobs(logits, tokens, out_logprob, *, out_entropy=None, out_rank=None, out_top_ids=None, out_top_logprobs=None) -> None:
+    """What each row of logits [R, V] (32-bit or bfloat16; rows may lie apart, as columns of a wider buffer) says about a token of
+    it: out_logprob[r] = log softmax(logits[r])[tokens[r]], out_rank[r] = the columns that come before the token (larger, or equal
+    with a lower id), out_entropy[r] = -sum p log p, and out_top_ids / out_top_logprobs [R, k] = the k most likely columns, the
+    lower id first among equals, k <= 64.  Any output but the first may be None; without tokens (None) that one is None too.
+    Results are 32-bit, of sums held in 32-bit.
+
+    A negative token leaves its row's outputs as they are (a row of padding).  A token of V or more gives NaN and rank -1.  Columns
+    of -inf are masked: they have no probability; a row of nothing else gives -inf and entropy 0.  A row with NaN or +inf gives NaN,
+    and NaN comes last among the alternatives."""
+    what = "token_logprobs"
+    if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16):
+        raise KernelError(f"{what}: logits are {tuple(logits.shape)} {logits.dtype}, not rows of float32 or bfloat16")
+    R, V = logits.shape
+    if V < 1 or (V > 1 and logits.stride(1) != 1):
+        raise KernelError(f"{what}: the columns of a row must lie side by side (strides {tuple(logits.stride())}, {V} columns)")
+    _check_tokens(what, tokens, R, out_logprob, out_rank)
+    _check_out(what, "out_entropy", out_entropy, (R,), torch.float32)
+    top = 0
+    for name, t, dtype in (("out_top_ids", out_top_ids, torch.int32), ("out_top_logprobs", out_top_logprobs, torch.float32)):
+        if t is not None:
+            k = t.shape[-1] if t.dim() else 0
+            if not 1 <= k <= min(MAX_TOP_LOGPROBS, V) or (top and k != top):
+                raise KernelError(f"{what}: {k} alternatives are not 1..min({MAX_TOP_LOGPROBS}, {V}), or not the same in both outputs")
+            top = k
+            _check_out(what, name, t, (R, k), dtype)
+    if out_logprob is None and out_entropy is None and out_rank is None and top == 0:
+        raise KernelError(f"{what}: nothing to compute")
+    outs = (out_logprob, out_entropy, out_rank, out_top_ids, out_top_logprobs)
+    _same_device(what, logits, tokens, *outs)
+    if R == 0:
+        return
+    if not logits.is_cuda:
+        _p(logits)                                          # refuses, with the reason
+    _check(library().kf_token_logprobs(ctypes.c_void_p(logits.data_ptr()), _dt(logits), ctypes.c_long(logits.stride(0)), R, V, _p(tokens),
+                                       _p(out_logprob), _p(out_entropy), _p(out_rank), top, _p(out_top_ids),
+                                       _p(out_top_logprobs), _stream()), what)
+
+
+LOGITS_PIECE_BYTES = 256 << 20  # logits held at a time where `head_logprobs` computes them first
+
+
+@_dispatch("head_logprobs")
+def head_logprobs(x, weight, tokens, out_logprob, *, out_entropy=None, softcap: float = 0.0) -> None:
+    """`token_logprobs` of the logits x[R, K] . weight[V, K]^T (cap * tanh(. / cap) of them where softcap > 0): the log probability of
+    tokens[r] and, if wanted, the entropy of every row, for programs that have no use for the logits themselves (2,048 rows over
+    256,000 columns: 2 GB).  The same rules for negative tokens, tokens of V or more, and rows without finite numbers."""
+    what = "head_logprobs"
+    if x.dim() != 2 or weight.dim() != 2 or x.shape[1] != weight.shape[1] or x.shape[1] < 1 or weight.shape[0] < 1:
+        raise KernelError(f"{what}: shapes x{tuple(x.shape)} w{tuple(weight.shape)} do not agree")
+    for t in (x, weight):
+        if t.dtype not in (torch.float32, torch.bfloat16) or not t.is_contiguous():
+            raise KernelError(f"{what}: x and weight are contiguous float32 or bfloat16 (got {t.dtype})")
+    if not 0.0 <= softcap < float("inf"):
+        raise KernelError(f"{what}: softcap {softcap} is not 0 or a positive number")
+    (R, K), V = x.shape, weight.shape[0]
+    if tokens is None or out_logprob is None:
+        raise KernelError(f"{what}: tokens and out_logprob are needed")
+    _check_tokens(what, tokens, R, out_logprob)
+    _check_out(what, "out_entropy", out_entropy, (R,), torch.float32)
+    _same_device(what, x, weight, tokens, out_logprob, out_entropy)
+    if R == 0:
+        return
+    if not x.is_cuda:
+        _p(x)
+    step = max(1, min(R, LOGITS_PIECE_BYTES // (4 * V)))
+    logits = torch.empty((step, V), dtype=torch.float32, device=x.device)
+    for a in range(0, R, step):
+        b = min(R, a + step)
+        linear(x[a:b], weight, logits[:b - a], softcap=softcap)
+        token_logprobs(logits[:b - a], tokens[a:b], out_logprob[a:b], out_entropy=None if out_entropy is None else out_entropy[a:b])
+
+
+@_dispatch("copy_pages")
+def copy_pages(stores, src, dst) -> None:
+    """In every store (a contiguous tensor whose first dimension counts pages, or rows of a per-request state): page dst[i] becomes
+    a copy of page src[i].  `src` and `dst` are host integers, as the cache manager's tables hold them.  No page may be named twice
+    as a destination, or be both a source and a destination: the copies run at the same time."""
+    what = "copy_pages"
+    stores = list(stores)
+    pairs = [(int(a), int(b)) for a, b in zip(src, dst)]
+    if len(pairs) != len(src) or len(pairs) != len(dst):
+        raise KernelError(f"{what}: {len(src)} sources for {len(dst)} destinations")
+    to = {b for _, b in pairs}
+    if len(to) != len(pairs) or any(a in to for a, _ in pairs):
+        raise KernelError(f"{what}: a page is a destination twice, or a source and a destination")
+    last = max((max(p) for p in pairs), default=-1)
+    if pairs and min(min(p) for p in pairs) < 0:
+        raise KernelError(f"{what}: a page below 0")
+    for t in stores:
+        if t.dim() < 1 or not t.is_contiguous() or t.shape[0] <= last:
+            raise KernelError(f"{what}: a store is contiguous and has more than {last} pages (got {tuple(t.shape)}, strides {tuple(t.stride())})")
+    _same_device(what, *stores)
+    live = [t for t in stores if t.numel()]
+    if not pairs or not live:
+        return
+    if not live[0].is_cuda:
+        _p(live[0])
+    lib = library()
+    for a in range(0, len(live), 64):
+        some = live[a:a + 64]
+        bases = (ctypes.c_int64 * len(some))(*[t.data_ptr() for t in some])
+        sizes = (ctypes.c_int64 * len(some))(*[t.numel() // t.shape[0] * t.element_size() for t in some])
+        for i in range(0, len(pairs), 256):
+            part = pairs[i:i + 256]
+            ids = (ctypes.c_int * len(part))
+            _check(lib.kf_copy_pages(bases, sizes, len(some), ids(*[p[0] for p in part]), ids(*[p[1] for p in part]), len(part),
+                                     _stream()), what)
+
+
 def device_arch() -> int:
     return int(library().kf_device_arch())

@@ -746,3 +746,34 @@ class CpuOps:
         out_ids.copy_(order.to(torch.int32))
         out_vals.copy_(torch.gather(logits, 1, order))
         out_lse.copy_(torch.logsumexp(logits.double(), dim=-1).float())
+
+    def token_logprobs(self, logits, tokens, out_logprob, *, out_entropy=None, out_rank=None, out_top_ids=None, out_top_logprobs=None):
+        x = logits.double()
+        lse = torch.logsumexp(x, dim=-1)
+        live = torch.ones(x.shape[0], dtype=torch.bool) if tokens is None else tokens >= 0
+        p = torch.exp(x - lse[:, None])
+        if out_entropy is not None:
+            out_entropy[live] = -torch.where(p > 0, p * (x - lse[:, None]), 0.0).sum(1).float()[live]
+        if tokens is not None:
+            t = tokens.long().clamp(min=0)[:, None]
+            xt = x.gather(1, t)
+            if out_logprob is not None:
+                out_logprob[live] = (xt[:, 0] - lse).float()[live]
+            if out_rank is not None:
+                ids = torch.arange(x.shape[1])[None, :]
+                out_rank[live] = ((x > xt) | ((x == xt) & (ids < t))).sum(1).to(torch.int32)[live]
+        for out in (out_top_ids, out_top_logprobs):
+            if out is not None:
+                order = torch.argsort(-x, dim=-1, stable=True)[:, :out.shape[1]]
+                vals = order.to(torch.int32) if out is out_top_ids else (x.gather(1, order) - lse[:, None]).float()
+                out[live] = vals[live]
+
+    def head_logprobs(self, x, weight, tokens, out_logprob, *, out_entropy=None, softcap=0.0):
+        logits = x.double() @ weight.double().T
+        if softcap > 0.0:
+            logits = softcap * torch.tanh(logits / softcap)
+        self.token_logprobs(logits, tokens, out_logprob, out_entropy=out_entropy)
+
+    def copy_pages(self, stores, src, dst):
+        for t in stores:
+            t[list(dst)] = t[list(src)].clone()
