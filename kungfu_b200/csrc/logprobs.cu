@@ -6,110 +6,515 @@
 //
 // Both terms of H are >= 0, so nothing cancels.  A row whose every column is -inf has no distribution: its log probabilities
 // are -inf and its entropy 0.  A row that holds NaN or +inf gives NaN.  NaN ranks behind -inf among the alternatives.
+//
+// Shape.  A row is read once.  A block walks its slice of the row in chunks of 8,192 columns, 32 in the registers of each
+// thread (the next chunk's on their way), and keeps per thread the running maximum m, s and u = sum d exp(d) (a new maximum moves
+// both: u' = f (u + (m - m') s), s' = f s, f = exp(m - m')).  A cluster of up to 16 blocks shares a row when there are few
+// rows; each leaves its numbers in the first block's shared memory, so nothing passes through a workspace and one launch does it all.
+// Alternatives: the block keeps a list of keys that can still be among its k best, in shared memory, and a value tau that a
+// column must exceed to join them.  The first chunk gives tau: a bound that at least k of its columns reach (`warp_bound`).  From
+// then on a column costs one comparison (of the thread's maximum); a warp that finds such a thread looks at that thread's 32
+// columns again, one per lane, out of the L1 cache.  A list grown long is pruned to its k best, which raises tau.
 #include "common.cuh"
 
 namespace {
 
 constexpr int TOP_MAX = 64;
+constexpr int NT = 256, WARPS = NT / 32;
+constexpr int PER_THREAD = 32;                               // columns of a chunk in a thread's registers
+constexpr int CHUNK = NT * PER_THREAD;
+constexpr int MAX_SLICES = 16;
+constexpr int KEY_CAP = NT * 8 + TOP_MAX;                    // keys held at most: a vector of every thread beside the k best
+constexpr int FEW_KEYS = 256;                                // up to here keys are ranked by counting the larger ones at once
+constexpr int LONG_LIST = 512;                               // a list beyond this is pruned
+constexpr float LOG2E = 1.4426950408889634f;
 
-// (order-preserving image of the value) << 32 | ~id: a larger key comes first, no two are equal, zero is none of them
-__device__ __forceinline__ unsigned long long rank_key(float v, unsigned id) {
-  unsigned b = __float_as_uint(v == 0.f ? 0.f : v);
-  b = v != v ? 0u : ((b & 0x80000000u) ? ~b : (b | 0x80000000u));
-  return ((unsigned long long)b << 32) | (unsigned long long)(0xFFFFFFFFu - id);
+typedef unsigned long long u64;
+
+__device__ __forceinline__ unsigned orderable(float v) {     // larger float <=> larger unsigned; -0 as +0; NaN below everything
+  const unsigned b = __float_as_uint(v == 0.f ? 0.f : v);
+  return v != v ? 0u : ((b & 0x80000000u) ? ~b : (b | 0x80000000u));
 }
-__device__ __forceinline__ float rank_value(unsigned long long key) {
+// (value, id) as one number: a larger key comes first, no two are equal, zero is none of them
+__device__ __forceinline__ u64 rank_key(float v, unsigned id) { return ((u64)orderable(v) << 32) | (u64)(0xFFFFFFFFu - id); }
+__device__ __forceinline__ float rank_value(u64 key) {
   const unsigned o = (unsigned)(key >> 32);
   return o == 0u ? __int_as_float(0x7fffffff) : __uint_as_float((o & 0x80000000u) ? (o & 0x7FFFFFFFu) : ~o);
 }
+__device__ __forceinline__ int rank_id(u64 key) { return (int)(0xFFFFFFFFu - (unsigned)key); }
 
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
 
-template <typename T>
-__global__ void __launch_bounds__(256)
+// Sixteen bytes of a row as floats
+template <typename T> struct Vec;
+template <> struct Vec<float> {
+  static constexpr int N = 4;
+  static constexpr unsigned MASKED = 0xff800000u;
+  static __device__ __forceinline__ float get(const uint4& v, int i) {
+    return __uint_as_float(i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w);
+  }
+};
+template <> struct Vec<__nv_bfloat16> {
+  static constexpr int N = 8;
+  static constexpr unsigned MASKED = 0xff80ff80u;
+  static __device__ __forceinline__ float get(const uint4& v, int i) {
+    const unsigned w = i < 2 ? v.x : i < 4 ? v.y : i < 6 ? v.z : v.w;
+    return __uint_as_float((i & 1) ? (w & 0xffff0000u) : (w << 16));
+  }
+};
+
+// Running maximum, sum of exponentials and sum of d exp(d), and how a second set joins the first.
+struct Stats { float m, s, u; };
+__device__ __forceinline__ void move_to(Stats& a, float m) {
+  if (m != a.m) {
+    const float d = a.m - m, f = exp2_fast(d * LOG2E);
+    a.u = a.s == 0.f ? 0.f : f * (a.u + d * a.s);
+    a.s *= f;
+    a.m = m;
+  }
+}
+__device__ __forceinline__ void join(Stats& a, Stats b) {
+  const float m = max_nan(a.m, b.m);
+  move_to(a, m);
+  move_to(b, m);
+  a.s += b.s;
+  a.u += b.u;
+}
+
+struct Shared {
+  Stats stats[WARPS];
+  int before[WARPS];
+  u64 bound[WARPS];
+  int n_keys;
+  u64 sorted[TOP_MAX];
+  u64 keys[KEY_CAP];
+};
+struct ClusterShared {                                        // what the row's blocks leave with the first one
+  Stats stats[MAX_SLICES];
+  int before[MAX_SLICES];
+  u64 keys[MAX_SLICES * TOP_MAX];
+};
+
+// A key that at least k of the block's thread maxima reach (0: there may be fewer): with q = ceil(k / warps), the smallest of
+// the warps' q-th largest.  A thread's rank in its warp is how many lanes hold more.  All threads call it.
+__device__ __forceinline__ u64 warp_bound(u64 mine, int k, Shared& sh) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int q = (k + WARPS - 1) / WARPS;
+  int rank = 0;
+#pragma unroll
+  for (int o = 1; o < 32; ++o) {
+    const u64 other = __shfl_sync(0xffffffffu, mine, (lane + o) & 31);
+    rank += (other > mine || (other == mine && ((lane + o) & 31) < lane)) ? 1 : 0;      // equal: only the absent ones (zero)
+  }
+  if (rank == q - 1) sh.bound[warp] = mine;
+  __syncthreads();
+  u64 b = sh.bound[0];
+#pragma unroll
+  for (int w = 1; w < WARPS; ++w) b = sh.bound[w] < b ? sh.bound[w] : b;
+  __syncthreads();
+  return b;
+}
+
+// The keys of sh.keys[0, n) that `keep` takes, moved to its front; returns how many.  All threads call it.
+template <typename F>
+__device__ __forceinline__ int compact(int n, Shared& sh, F keep) {
+  constexpr int MINE = (KEY_CAP + NT - 1) / NT;
+  const int tid = threadIdx.x;
+  u64 mine[MINE];
+#pragma unroll
+  for (int j = 0; j < MINE; ++j) mine[j] = tid + j * NT < n ? sh.keys[tid + j * NT] : 0ull;
+  __syncthreads();
+  if (tid == 0) sh.n_keys = 0;
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < MINE; ++j)
+    if (mine[j] != 0ull && keep(mine[j])) sh.keys[atomicAdd(&sh.n_keys, 1)] = mine[j];
+  __syncthreads();
+  return sh.n_keys;
+}
+
+// The k best of keys[0, n) to sh.sorted, in order: a key's place is how many are larger; `share` neighbouring lanes count for
+// one key.  Zeros are absent ones.  All threads call it.
+__device__ __forceinline__ void rank_keys(const u64* keys, int n, int k, Shared& sh) {
+  int share = 1;
+  while (share < 8 && n * share * 2 <= NT) share *= 2;
+  for (int i0 = 0; i0 * share < n * share; i0 += NT / share) {
+    const int i = i0 + threadIdx.x / share;
+    const u64 key = i < n ? keys[i] : 0ull;
+    int rank = 0;
+#pragma unroll 4
+    for (int j = threadIdx.x % share; j < n; j += share) rank += keys[j] > key ? 1 : 0;
+    for (int o = 1; o < share; o *= 2) rank += __shfl_xor_sync(0xffffffffu, rank, o);
+    if (key != 0ull && rank < k && threadIdx.x % share == 0) sh.sorted[rank] = key;
+  }
+  __syncthreads();
+}
+
+// The k best of the n keys held, in order, to sh.sorted and back to the list; returns how many there are.  All threads call it.
+__device__ __noinline__ int prune(int n, int k, Shared& sh) {
+  const int tid = threadIdx.x;
+  if (n > FEW_KEYS) {                                         // first only those that reach a bound of the threads' maxima
+    u64 best = 0ull;
+    for (int i = tid; i < n; i += NT) best = sh.keys[i] > best ? sh.keys[i] : best;
+    const u64 bound = warp_bound(best, k, sh);
+    n = compact(n, sh, [&](u64 key) { return key >= bound; });
+  }
+  rank_keys(sh.keys, n, k, sh);
+  const int kept = min(n, k);
+  if (tid < kept) sh.keys[tid] = sh.sorted[tid];
+  if (tid == 0) sh.n_keys = kept;
+  __syncthreads();
+  return kept;
+}
+
+template <typename T, bool RANK, bool TOP>
+__global__ void __launch_bounds__(NT, 2)
 token_logprobs_kernel(const T* __restrict__ logits, long ld, int V, const int* __restrict__ tokens, float* __restrict__ logprob,
-                      float* __restrict__ entropy, int* __restrict__ rank, int top, int* __restrict__ top_ids,
-                      float* __restrict__ top_logprobs) {
+                      float* __restrict__ entropy, int* __restrict__ rank_out, int top, int* __restrict__ top_ids,
+                      float* __restrict__ top_logprobs, int slices) {
+  constexpr int VN = Vec<T>::N, NV = PER_THREAD / VN, STEP = NT * NV;
+  extern __shared__ __align__(16) unsigned char cluster_raw[];       // a ClusterShared where a cluster shares a row
+  __shared__ Shared sh;
   kf_pdl_trigger();
+  if (slices > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");      // waited for before a peer's memory is touched
   kf_pdl_wait();
-  __shared__ float red[33];
-  __shared__ unsigned long long best[8];
-  const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int row = (int)(blockIdx.x / (unsigned)slices), slice = (int)(blockIdx.x % (unsigned)slices);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int token = tokens ? tokens[row] : 0;
-  if (token < 0) return;                                    // a row of padding
+  if (token < 0) return;                                      // a row of padding: its whole cluster leaves
   const T* x = logits + (size_t)row * ld;
   const bool inside = token < V;
-  float m = -INFINITY;
-  for (int i = tid; i < V; i += 256) m = max_nan(m, kf_load(x, i));
+
+  // The row: `head` elements up to a 16-byte boundary, `n_vec` vectors, the rest.  Loose elements go to the first slice.
+  const int head = min(V, (int)((16 - ((uintptr_t)x & 15)) % 16 / sizeof(T)));
+  const int n_vec = (V - head) / VN, loose = V - n_vec * VN;
+  const T* body = x + head;
+  const int per = (n_vec + slices - 1) / slices;
+  const int v_begin = min(n_vec, slice * per), v_end = min(n_vec, v_begin + per);
+
+  auto load = [&](int c, uint4 (&raw)[NV]) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-  if (lane == 0) red[warp] = m;
-  __syncthreads();
-  for (int w = 0; w < 8; ++w) m = max_nan(m, red[w]);
+    for (int j = 0; j < NV; ++j) {
+      const int v = c + j * NT + tid;
+      raw[j] = make_uint4(Vec<T>::MASKED, Vec<T>::MASKED, Vec<T>::MASKED, Vec<T>::MASKED);
+      if (v < v_end) raw[j] = __ldg(reinterpret_cast<const uint4*>(body) + v);
+    }
+  };
+  uint4 raw[NV];
+  load(v_begin, raw);
   const float given = inside ? kf_load(x, token) : 0.f;
-  float s = 0.f, u = 0.f, before = 0.f;
-  for (int i = tid; i < V; i += 256) {
-    const float v = kf_load(x, i), d = v - m;
-    const float e = m == -INFINITY ? 0.f : expf(d);
-    s += e;
-    if (e > 0.f) u += d * e;
-    before += (v > given || (v == given && i < token)) ? 1.f : 0.f;
+
+  Stats st = {-INFINITY, 0.f, 0.f};
+  int before = 0;
+  bool open = true;                                           // fewer than `top` keys are known: there is no tau yet
+  float tau = -INFINITY;
+  if (TOP && tid == 0) sh.n_keys = slice == 0 ? loose : 0;
+  if (slice == 0 && tid < loose) {
+    const int i = tid < head ? tid : n_vec * VN + tid;
+    const float v = kf_load(x, i);
+    st.m = v;
+    st.s = v == -INFINITY ? 0.f : 1.f;
+    if (RANK) before = (v > given || (v == given && i < token)) ? 1 : 0;
+    if (TOP) sh.keys[tid] = rank_key(v, (unsigned)i);
   }
-  s = kf_block_sum(s, red);
-  u = kf_block_sum(u, red);
-  const float n_before = kf_block_sum(before, red);
-  const bool empty = m == -INFINITY;
-  const float log_s = logf(s);
-  if (tid == 0) {
-    if (logprob) logprob[row] = !inside ? __int_as_float(0x7fffffff) : (empty ? -INFINITY : (given - m) - log_s);
-    if (entropy) entropy[row] = empty ? 0.f : log_s - u / s;
-    if (rank) rank[row] = inside ? (int)n_before : -1;
-  }
-  unsigned long long last = ~0ull;
-  for (int k = 0; k < top; ++k) {
-    unsigned long long b = 0ull;
-    for (int i = tid; i < V; i += 256) {
-      const unsigned long long key = rank_key(kf_load(x, i), (unsigned)i);
-      if (key < last && key > b) b = key;
+
+#pragma unroll 1
+  for (int c = v_begin; c < v_end; c += STEP) {
+    uint4 next[NV];
+    load(c + STEP, next);                                     // (nothing is read beyond the slice)
+    float cm = Vec<T>::get(raw[0], 0);
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int e = 0; e < VN; ++e) cm = max_nan(cm, Vec<T>::get(raw[j], e));
+    move_to(st, max_nan(st.m, cm));
+    {
+      const float ref = st.m == -INFINITY ? 0.f : st.m;
+      float s[2] = {0.f, 0.f}, u[2] = {0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int e = 0; e < VN; ++e) {
+          const float d = fmaxf(Vec<T>::get(raw[j], e) - ref, -200.f);      // exp(-200) is 0 in 32 bits, and 0 * -200 is 0
+          const float w = exp2_fast(d * LOG2E);
+          s[e & 1] += w;
+          u[e & 1] = fmaf(d, w, u[e & 1]);
+        }
+      st.s += s[0] + s[1];
+      st.u += u[0] + u[1];
+    }
+    if (RANK) {
+      // columns before the token count when they equal it, columns behind it do not: one comparison, unless the chunk holds the
+      // token or ends early (its masked places are no columns)
+      const long i_begin = (long)c * VN + head;
+      const bool whole = c + STEP <= v_end;
+      if (whole && i_begin + CHUNK <= token) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+          for (int e = 0; e < VN; ++e) before += Vec<T>::get(raw[j], e) >= given ? 1 : 0;
+      } else if (i_begin > token) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+          for (int e = 0; e < VN; ++e) before += Vec<T>::get(raw[j], e) > given ? 1 : 0;
+      } else {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+          const int v = c + j * NT + tid;
+          const int earlier = v < v_end ? (int)min((long)VN, (long)token - ((long)v * VN + head)) : 0;       // elements before the token
+#pragma unroll
+          for (int e = 0; e < VN; ++e) {
+            const float value = Vec<T>::get(raw[j], e);
+            before += (value > given || (value == given && e < earlier)) ? 1 : 0;
+          }
+        }
+      }
+    }
+    if (TOP) {
+      // The warp looks at the 32 columns of each of its lanes in `who`, one per lane, and pushes those `takes` takes; returns the
+      // longest list it saw.  A key that finds the list full is not written, and the length tells.
+      auto push = [&](unsigned who, auto takes) {
+        int seen = 0;
+        while (who) {
+          const int of = __ffs(who) - 1;
+          who &= who - 1;
+          const int v = c + (lane / VN) * NT + warp * 32 + of;
+          const bool here = v < v_end;
+          const long i = (long)v * VN + lane % VN;
+          const float value = here ? kf_load(body, i) : 0.f;
+          const unsigned id = (unsigned)(i + head);
+          const bool hit = here && takes(value, id);
+          const unsigned hits = __ballot_sync(0xffffffffu, hit);
+          if (hits) {
+            int at = 0;
+            if (lane == 0) at = atomicAdd(&sh.n_keys, __popc(hits));
+            at = __shfl_sync(0xffffffffu, at, 0);
+            seen = at + __popc(hits);
+            at += __popc(hits & ((1u << lane) - 1u));
+            if (hit && at < KEY_CAP) sh.keys[at] = rank_key(value, id);
+          }
+        }
+        return seen;
+      };
+      auto settle = [&](int n) {                              // after a prune
+        tau = n < top ? -INFINITY : rank_value(sh.keys[top - 1]);
+        open = n < top || tau != tau;                         // (NaN is the least there is: everything comes before it)
+        __syncthreads();
+      };
+      int seen = 0;
+      if (!open) seen = push(__ballot_sync(0xffffffffu, !(cm <= tau)), [&](float v, unsigned) { return v > tau; });
+      if (__syncthreads_or(open || seen > LONG_LIST)) {
+        int n = sh.n_keys;
+        const bool full = n > KEY_CAP;
+        __syncthreads();
+        if (!open && !full) {
+          settle(prune(n, top, sh));
+        } else {
+          // The first chunk, or one that brought more than the list holds: cut it by its own bound.  Keys of this chunk that are in the
+          // list already go first.
+          const unsigned id0 = (unsigned)(c * (long)VN + head), id1 = (unsigned)(min(v_end, c + STEP) * (long)VN + head);
+          auto older = [&](u64 key) { return (unsigned)rank_id(key) < id0 || (unsigned)rank_id(key) >= id1; };
+          if (full) {
+            n = compact(KEY_CAP, sh, older);
+            if (n >= top) settle(prune(n, top, sh));
+          }
+          int e_best = -1;                                    // the first of the thread's columns that is its maximum
+#pragma unroll
+          for (int j = NV - 1; j >= 0; --j)
+#pragma unroll
+            for (int e = VN - 1; e >= 0; --e)
+              if (Vec<T>::get(raw[j], e) == cm) e_best = j * VN + e;
+          const int v_best = c + e_best / VN * NT + tid;
+          u64 best = 0ull;
+          if (e_best >= 0 && v_best < v_end && (open || cm > tau)) best = rank_key(cm, (unsigned)((long)v_best * VN + e_best % VN + head));
+          const u64 bound = warp_bound(best, top, sh);
+          const bool was_open = open;
+          const float was_tau = tau;
+          auto takes = [&](float v, unsigned id) { return (was_open || v > was_tau) && rank_key(v, id) >= bound; };
+          push(__ballot_sync(0xffffffffu, bound == 0ull || best >= bound || cm != cm), takes);      // (NaN hides a thread's maximum)
+          __syncthreads();
+          n = sh.n_keys;
+          __syncthreads();
+          if (n <= KEY_CAP) {
+            if (bound != 0ull) {                              // at least `top` columns reach it
+              tau = rank_value(bound);
+              open = false;
+            } else if (n >= top) {
+              settle(prune(n, top, sh));
+            }
+          } else {                                            // still too many (a chunk full of NaN): one vector of each thread at a time
+            n = compact(KEY_CAP, sh, older);
+#pragma unroll 1
+            for (int j = 0; j < NV; ++j) {
+              const int v = c + j * NT + tid;
+              if (v < v_end)
+#pragma unroll 1
+                for (int e = 0; e < VN; ++e) {
+                  const long i = (long)v * VN + e;
+                  const float value = kf_load(body, i);
+                  if (open || value > tau) sh.keys[atomicAdd(&sh.n_keys, 1)] = rank_key(value, (unsigned)(i + head));
+                }
+              __syncthreads();
+              n = sh.n_keys;
+              __syncthreads();
+              settle(prune(n, top, sh));
+            }
+          }
+        }
+      }
     }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const unsigned long long other = __shfl_xor_sync(0xffffffffu, b, o);
-      b = other > b ? other : b;
-    }
+    for (int j = 0; j < NV; ++j) raw[j] = next[j];
+  }
+
+  // the block's numbers, then the cluster's
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    Stats other = {__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.s, o), __shfl_xor_sync(0xffffffffu, st.u, o)};
+    join(st, other);
+    if (RANK) before += __shfl_xor_sync(0xffffffffu, before, o);
+  }
+  if (lane == 0) {
+    sh.stats[warp] = st;
+    sh.before[warp] = before;
+  }
+  __syncthreads();
+  int n = 0;
+  if (TOP) {
+    n = sh.n_keys;                                            // within the list's room after every chunk
     __syncthreads();
-    if (lane == 0) best[warp] = b;
-    __syncthreads();
-    for (int w = 0; w < 8; ++w) b = best[w] > b ? best[w] : b;
-    last = b;
+    n = prune(n, top, sh);
+  }
+  st = sh.stats[0];
+  before = sh.before[0];
+#pragma unroll
+  for (int w = 1; w < WARPS; ++w) {
+    join(st, sh.stats[w]);
+    before += sh.before[w];
+  }
+  if (slices > 1) {
+    const uint32_t mine = (uint32_t)__cvta_generic_to_shared(cluster_raw);
+    uint32_t first;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(first) : "r"(mine));
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");                       // every block of the row has begun
     if (tid == 0) {
-      const float v = rank_value(b);
-      if (top_ids) top_ids[(size_t)row * top + k] = (int)(0xFFFFFFFFu - (unsigned)b);
-      if (top_logprobs) top_logprobs[(size_t)row * top + k] = (empty && v == v) ? -INFINITY : (v - m) - log_s;
+      const uint32_t at = first + (uint32_t)offsetof(ClusterShared, stats) + (uint32_t)(sizeof(Stats) * slice);
+      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(st.m) : "memory");
+      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at + 4), "f"(st.s) : "memory");
+      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at + 8), "f"(st.u) : "memory");
+      asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(first + (uint32_t)offsetof(ClusterShared, before) + 4u * slice), "r"(before) : "memory");
     }
+    if (TOP && tid < top)
+      asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(first + (uint32_t)offsetof(ClusterShared, keys) + 8u * (slice * top + tid)),
+                   "l"(tid < n ? sh.sorted[tid] : 0ull) : "memory");
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (slice != 0) return;
+    const ClusterShared& all = *reinterpret_cast<const ClusterShared*>(cluster_raw);
+    st = all.stats[0];
+    before = all.before[0];
+    for (int r = 1; r < slices; ++r) {
+      join(st, all.stats[r]);
+      before += all.before[r];
+    }
+    if (TOP) {
+      for (int i = tid; i < slices * top; i += NT) sh.keys[i] = all.keys[i];
+      __syncthreads();
+      prune(slices * top, top, sh);
+    }
+  }
+  if (st.m == INFINITY) st.m = __int_as_float(0x7fffffff);
+  const bool empty = st.m == -INFINITY;
+  const float log_s = logf(st.s);
+  if (tid == 0) {
+    if (logprob) logprob[row] = !inside ? __int_as_float(0x7fffffff) : (empty ? -INFINITY : (given - st.m) - log_s);
+    if (entropy) entropy[row] = empty ? 0.f : log_s - st.u / st.s;
+    if (RANK) rank_out[row] = inside ? before : -1;
+  }
+  if (TOP && tid < top) {
+    const u64 key = sh.sorted[tid];
+    const float v = rank_value(key);
+    if (top_ids) top_ids[(size_t)row * top + tid] = rank_id(key);
+    if (top_logprobs) top_logprobs[(size_t)row * top + tid] = (empty && v == v) ? -INFINITY : (v - st.m) - log_s;
   }
 }
 
+template <typename T, bool RANK, bool TOP>
+int launch(const void* logits, long ld, int R, int V, const int* tokens, float* logprob, float* entropy, int* rank, int top,
+           int* top_ids, float* top_logprobs, int slices, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)R * (unsigned)slices);
+  cfg.blockDim = dim3(NT);
+  cfg.stream = stream;
+  cfg.dynamicSmemBytes = slices > 1 ? sizeof(ClusterShared) : 0;
+  if (slices > 8) {
+    static bool allowed[64] = {};                             // by device
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64 || !allowed[dev]) {
+      if (cudaFuncSetAttribute(token_logprobs_kernel<T, RANK, TOP>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
+        kf_record_cuda_error(cudaGetLastError());
+        return KF_ERR_SETUP;
+      }
+      if (dev >= 0 && dev < 64) allowed[dev] = true;
+    }
+  }
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)slices;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = kf_pdl_enabled() ? 2 : 1;
+  cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, RANK, TOP>, (const T*)logits, ld, V, tokens, logprob, entropy, rank, top, top_ids,
+                     top_logprobs, slices);
+  KF_CHECK_LAUNCH();
+  return KF_OK;
+}
+
+template <typename T>
+int launch_type(const void* logits, long ld, int R, int V, const int* tokens, float* logprob, float* entropy, int* rank, int top,
+                int* top_ids, float* top_logprobs, int slices, cudaStream_t stream) {
+  if (rank && top) return launch<T, true, true>(logits, ld, R, V, tokens, logprob, entropy, rank, top, top_ids, top_logprobs, slices, stream);
+  if (rank) return launch<T, true, false>(logits, ld, R, V, tokens, logprob, entropy, rank, top, top_ids, top_logprobs, slices, stream);
+  if (top) return launch<T, false, true>(logits, ld, R, V, tokens, logprob, entropy, rank, top, top_ids, top_logprobs, slices, stream);
+  return launch<T, false, false>(logits, ld, R, V, tokens, logprob, entropy, rank, top, top_ids, top_logprobs, slices, stream);
+}
+
 }  // namespace
+
+#ifdef KF_TUNING
+static int g_slices = 0;
+KF_API void kf_token_logprobs_slices(int n) { g_slices = n; }
+#endif
 
 // logits [R, V] of element type dt (KF_F32, KF_BF16), rows ld elements apart; tokens [R] (null: only entropy and alternatives;
 // a negative one: the row's outputs stay as they are; one >= V: NaN and rank -1); every output may be null; top <= 64, <= V.
 KF_API int kf_token_logprobs(const void* logits, int dt, long ld, int R, int V, const int* tokens, float* logprob, float* entropy,
                              int* rank, int top, int* top_ids, float* top_logprobs, cudaStream_t stream) {
   if (R <= 0) return KF_OK;
-  if (V <= 0 || top < 0 || top > TOP_MAX || top > V || (!tokens && (logprob || rank))) return KF_ERR_SIZE;
+  if (V <= 0 || V > 0x7fffff00 || R > (1 << 27) || top < 0 || top > TOP_MAX || top > V || (!tokens && (logprob || rank))) return KF_ERR_SIZE;
+  if (((uintptr_t)logits & (dt == KF_F32 ? 3 : 1)) != 0) return KF_ERR_ALIGN;
+  // Blocks for every SM twice over, but no slice below a chunk.
+  const int chunks = kf_ceil_div(V, CHUNK);
+  int slices = 1;
+  while (slices < MAX_SLICES && slices < chunks && (long)R * slices < 2l * kf_sm_count()) slices *= 2;
+#ifdef KF_TUNING
+  if (g_slices > 0) slices = g_slices;
+#endif
   if (dt == KF_F32)
-    kf_launch(token_logprobs_kernel<float>, dim3(R), dim3(256), 0, stream, (const float*)logits, ld, V, tokens, logprob, entropy,
-              rank, top, top_ids, top_logprobs);
-  else if (dt == KF_BF16)
-    kf_launch(token_logprobs_kernel<__nv_bfloat16>, dim3(R), dim3(256), 0, stream, (const __nv_bfloat16*)logits, ld, V, tokens,
-              logprob, entropy, rank, top, top_ids, top_logprobs);
-  else
-    return KF_ERR_DTYPE;
-  KF_CHECK_LAUNCH();
-  return KF_OK;
+    return launch_type<float>(logits, ld, R, V, tokens, logprob, entropy, rank, top, top_ids, top_logprobs, slices, stream);
+  if (dt == KF_BF16)
+    return launch_type<__nv_bfloat16>(logits, ld, R, V, tokens, logprob, entropy, rank, top, top_ids, top_logprobs, slices, stream);
+  return KF_ERR_DTYPE;
 }
