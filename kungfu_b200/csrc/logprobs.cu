@@ -12,9 +12,9 @@
 // both: u' = f (u + (m - m') s), s' = f s, f = exp(m - m')).  A cluster of up to 16 blocks shares a row when there are few
 // rows; each leaves its numbers in the first block's shared memory, so nothing passes through a workspace and one launch does it all.
 // Alternatives: the block keeps a list of keys that can still be among its k best, in shared memory, and a value tau that a
-// column must exceed to join them.  The first chunk gives tau: a bound that at least k of its columns reach (`warp_bound`).  From
-// then on a column costs one comparison (of the thread's maximum); a warp that finds such a thread looks at that thread's 32
-// columns again, one per lane, out of the L1 cache.  A list grown long is pruned to its k best, which raises tau.
+// column must exceed to join them.  The first chunk is cut by a bound that at least k of its columns reach (`warp_bound`) and
+// leaves the exact k-th value as tau.  From then on a column costs one comparison (of the thread's maximum), and a random row
+// brings k * 8,192 / (columns seen) keys a chunk; a list grown long is pruned to its k best, which raises tau.
 #include "common.cuh"
 
 namespace {
@@ -26,7 +26,6 @@ constexpr int CHUNK = NT * PER_THREAD;
 constexpr int MAX_SLICES = 16;
 constexpr int KEY_CAP = NT * 8 + TOP_MAX;                    // keys held at most: a vector of every thread beside the k best
 constexpr int FEW_KEYS = 256;                                // up to here keys are ranked by counting the larger ones at once
-constexpr int LONG_LIST = 512;                               // a list beyond this is pruned
 constexpr float LOG2E = 1.4426950408889634f;
 
 typedef unsigned long long u64;
@@ -54,6 +53,33 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return r;
 }
 
+// Two 32-bit numbers in one instruction each (sm_100a)
+__device__ __forceinline__ u64 pack2(float a, float b) {
+  u64 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpack2(u64 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ u64 add2(u64 a, u64 b) {
+  u64 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ u64 mul2(u64 a, u64 b) {
+  u64 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ u64 fma2(u64 a, u64 b, u64 c) {
+  u64 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
 // Sixteen bytes of a row as floats
 template <typename T> struct Vec;
 template <> struct Vec<float> {
@@ -62,6 +88,7 @@ template <> struct Vec<float> {
   static __device__ __forceinline__ float get(const uint4& v, int i) {
     return __uint_as_float(i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w);
   }
+  static __device__ __forceinline__ float half_of(unsigned word, int) { return __uint_as_float(word); }
 };
 template <> struct Vec<__nv_bfloat16> {
   static constexpr int N = 8;
@@ -70,7 +97,24 @@ template <> struct Vec<__nv_bfloat16> {
     const unsigned w = i < 2 ? v.x : i < 4 ? v.y : i < 6 ? v.z : v.w;
     return __uint_as_float((i & 1) ? (w & 0xffff0000u) : (w << 16));
   }
+  static __device__ __forceinline__ float half_of(unsigned word, int i) { return __uint_as_float((i & 1) ? (word & 0xffff0000u) : (word << 16)); }
 };
+// Column `at` (0..31) of those a thread holds: a tree of selections, since registers have no addresses
+template <typename T, int NV>
+__device__ __forceinline__ float pick(const uint4 (&raw)[NV], int at) {
+  constexpr int PER_WORD = 4 / sizeof(T);
+  unsigned w[NV * 4];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) { w[4 * j] = raw[j].x; w[4 * j + 1] = raw[j].y; w[4 * j + 2] = raw[j].z; w[4 * j + 3] = raw[j].w; }
+  int word = at / PER_WORD;
+#pragma unroll
+  for (int n = NV * 4; n > 1; n /= 2) {
+#pragma unroll
+    for (int i = 0; i < n / 2; ++i) w[i] = (word & 1) ? w[2 * i + 1] : w[2 * i];
+    word >>= 1;
+  }
+  return Vec<T>::half_of(w[0], at);
+}
 
 // Running maximum, sum of exponentials and sum of d exp(d), and how a second set joins the first.
 struct Stats { float m, s, u; };
@@ -93,7 +137,7 @@ __device__ __forceinline__ void join(Stats& a, Stats b) {
 struct Shared {
   Stats stats[WARPS];
   int before[WARPS];
-  u64 bound[WARPS];
+  float bound[WARPS];
   int n_keys;
   u64 sorted[TOP_MAX];
   u64 keys[KEY_CAP];
@@ -104,29 +148,30 @@ struct ClusterShared {                                        // what the row's 
   u64 keys[MAX_SLICES * TOP_MAX];
 };
 
-// A key that at least k of the block's thread maxima reach (0: there may be fewer): with q = ceil(k / warps), the smallest of
-// the warps' q-th largest.  A thread's rank in its warp is how many lanes hold more.  All threads call it.
-__device__ __forceinline__ u64 warp_bound(u64 mine, int k, Shared& sh) {
+// A value that at least k of the block's threads' numbers reach (-inf: there may be fewer): with q = ceil(k / warps), the smallest
+// of the warps' q-th largest.  A number's rank in its warp is how many lanes hold a larger one, lower lanes first among equals.
+// All threads call it.
+__device__ __noinline__ float warp_bound(float mine, int k, Shared& sh) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int q = (k + WARPS - 1) / WARPS;
   int rank = 0;
 #pragma unroll
   for (int o = 1; o < 32; ++o) {
-    const u64 other = __shfl_sync(0xffffffffu, mine, (lane + o) & 31);
-    rank += (other > mine || (other == mine && ((lane + o) & 31) < lane)) ? 1 : 0;      // equal: only the absent ones (zero)
+    const float other = __shfl_sync(0xffffffffu, mine, (lane + o) & 31);
+    rank += (other > mine || (other == mine && ((lane + o) & 31) < lane)) ? 1 : 0;
   }
   if (rank == q - 1) sh.bound[warp] = mine;
   __syncthreads();
-  u64 b = sh.bound[0];
+  float b = sh.bound[0];
 #pragma unroll
-  for (int w = 1; w < WARPS; ++w) b = sh.bound[w] < b ? sh.bound[w] : b;
+  for (int w = 1; w < WARPS; ++w) b = fminf(b, sh.bound[w]);
   __syncthreads();
   return b;
 }
 
-// The keys of sh.keys[0, n) that `keep` takes, moved to its front; returns how many.  All threads call it.
-template <typename F>
-__device__ __forceinline__ int compact(int n, Shared& sh, F keep) {
+// Of the keys in the list [0, n), those of at least `bound` and whose ids are not in [id0, id1), moved to its front; returns how
+// many.  All threads call it.
+__device__ __noinline__ int compact(int n, float bound, unsigned id0, unsigned id1, Shared& sh) {
   constexpr int MINE = (KEY_CAP + NT - 1) / NT;
   const int tid = threadIdx.x;
   u64 mine[MINE];
@@ -136,10 +181,14 @@ __device__ __forceinline__ int compact(int n, Shared& sh, F keep) {
   if (tid == 0) sh.n_keys = 0;
   __syncthreads();
 #pragma unroll
-  for (int j = 0; j < MINE; ++j)
-    if (mine[j] != 0ull && keep(mine[j])) sh.keys[atomicAdd(&sh.n_keys, 1)] = mine[j];
+  for (int j = 0; j < MINE; ++j) {
+    const unsigned id = (unsigned)rank_id(mine[j]);
+    if (mine[j] != 0ull && rank_value(mine[j]) >= bound && (id < id0 || id >= id1)) sh.keys[atomicAdd(&sh.n_keys, 1)] = mine[j];
+  }
   __syncthreads();
-  return sh.n_keys;
+  const int left = sh.n_keys;
+  __syncthreads();
+  return left;
 }
 
 // The k best of keys[0, n) to sh.sorted, in order: a key's place is how many are larger; `share` neighbouring lanes count for
@@ -163,10 +212,10 @@ __device__ __forceinline__ void rank_keys(const u64* keys, int n, int k, Shared&
 __device__ __noinline__ int prune(int n, int k, Shared& sh) {
   const int tid = threadIdx.x;
   if (n > FEW_KEYS) {                                         // first only those that reach a bound of the threads' maxima
-    u64 best = 0ull;
-    for (int i = tid; i < n; i += NT) best = sh.keys[i] > best ? sh.keys[i] : best;
-    const u64 bound = warp_bound(best, k, sh);
-    n = compact(n, sh, [&](u64 key) { return key >= bound; });
+    float best = -INFINITY;
+    for (int i = tid; i < n; i += NT) best = fmaxf(best, rank_value(sh.keys[i]));
+    const float bound = warp_bound(best, k, sh);
+    n = compact(n, bound, 0u, 0u, sh);
   }
   rank_keys(sh.keys, n, k, sh);
   const int kept = min(n, k);
@@ -212,19 +261,23 @@ token_logprobs_kernel(const T* __restrict__ logits, long ld, int V, const int* _
   uint4 raw[NV];
   load(v_begin, raw);
   const float given = inside ? kf_load(x, token) : 0.f;
+  const float given_below = nextafterf(given, -INFINITY);
 
   Stats st = {-INFINITY, 0.f, 0.f};
   int before = 0;
-  bool open = true;                                           // fewer than `top` keys are known: there is no tau yet
-  float tau = -INFINITY;
-  if (TOP && tid == 0) sh.n_keys = slice == 0 ? loose : 0;
+  const int long_list = 2 * top + 64;                         // a list beyond this is pruned
+  float tau = -INFINITY;                                      // what a column must exceed to be a key; masked columns and NaN never are
+  if (TOP) {
+    if (tid == 0) sh.n_keys = 0;
+    __syncthreads();
+  }
   if (slice == 0 && tid < loose) {
     const int i = tid < head ? tid : n_vec * VN + tid;
     const float v = kf_load(x, i);
     st.m = v;
     st.s = v == -INFINITY ? 0.f : 1.f;
     if (RANK) before = (v > given || (v == given && i < token)) ? 1 : 0;
-    if (TOP) sh.keys[tid] = rank_key(v, (unsigned)i);
+    if (TOP && v > tau) sh.keys[atomicAdd(&sh.n_keys, 1)] = rank_key(v, (unsigned)i);
   }
 
 #pragma unroll 1
@@ -239,34 +292,34 @@ token_logprobs_kernel(const T* __restrict__ logits, long ld, int V, const int* _
     move_to(st, max_nan(st.m, cm));
     {
       const float ref = st.m == -INFINITY ? 0.f : st.m;
-      float s[2] = {0.f, 0.f}, u[2] = {0.f, 0.f};
+      const u64 minus = pack2(-ref, -ref), scale = pack2(LOG2E, LOG2E);
+      u64 s2 = 0ull, u2 = 0ull;
 #pragma unroll
       for (int j = 0; j < NV; ++j)
 #pragma unroll
-        for (int e = 0; e < VN; ++e) {
-          const float d = fmaxf(Vec<T>::get(raw[j], e) - ref, -200.f);      // exp(-200) is 0 in 32 bits, and 0 * -200 is 0
-          const float w = exp2_fast(d * LOG2E);
-          s[e & 1] += w;
-          u[e & 1] = fmaf(d, w, u[e & 1]);
+        for (int e = 0; e < VN; e += 2) {
+          float2 d = unpack2(add2(pack2(Vec<T>::get(raw[j], e), Vec<T>::get(raw[j], e + 1)), minus));
+          const u64 low = pack2(fmaxf(d.x, -200.f), fmaxf(d.y, -200.f));    // exp(-200) is 0 in 32 bits, and 0 * -200 is 0
+          d = unpack2(mul2(low, scale));
+          const u64 w = pack2(exp2_fast(d.x), exp2_fast(d.y));
+          s2 = add2(s2, w);
+          u2 = fma2(low, w, u2);
         }
-      st.s += s[0] + s[1];
-      st.u += u[0] + u[1];
+      const float2 s = unpack2(s2), u = unpack2(u2);
+      st.s += s.x + s.y;
+      st.u += u.x + u.y;
     }
     if (RANK) {
-      // columns before the token count when they equal it, columns behind it do not: one comparison, unless the chunk holds the
-      // token or ends early (its masked places are no columns)
+      // Columns before the token count when they equal it, columns behind it do not: they must exceed the next lower number, or the
+      // token's own.  One by one where the chunk holds the token, ends early (its masked places are no columns) or the token is masked.
       const long i_begin = (long)c * VN + head;
-      const bool whole = c + STEP <= v_end;
-      if (whole && i_begin + CHUNK <= token) {
+      const bool behind = i_begin > token;
+      if (behind || (c + STEP <= v_end && i_begin + CHUNK <= token && given > -INFINITY)) {
+        const float over = behind ? given : given_below;
 #pragma unroll
         for (int j = 0; j < NV; ++j)
 #pragma unroll
-          for (int e = 0; e < VN; ++e) before += Vec<T>::get(raw[j], e) >= given ? 1 : 0;
-      } else if (i_begin > token) {
-#pragma unroll
-        for (int j = 0; j < NV; ++j)
-#pragma unroll
-          for (int e = 0; e < VN; ++e) before += Vec<T>::get(raw[j], e) > given ? 1 : 0;
+          for (int e = 0; e < VN; ++e) before += Vec<T>::get(raw[j], e) > over ? 1 : 0;
       } else {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
@@ -281,96 +334,81 @@ token_logprobs_kernel(const T* __restrict__ logits, long ld, int V, const int* _
       }
     }
     if (TOP) {
-      // The warp looks at the 32 columns of each of its lanes in `who`, one per lane, and pushes those `takes` takes; returns the
-      // longest list it saw.  A key that finds the list full is not written, and the length tells.
-      auto push = [&](unsigned who, auto takes) {
-        int seen = 0;
-        while (who) {
-          const int of = __ffs(who) - 1;
-          who &= who - 1;
-          const int v = c + (lane / VN) * NT + warp * 32 + of;
-          const bool here = v < v_end;
-          const long i = (long)v * VN + lane % VN;
-          const float value = here ? kf_load(body, i) : 0.f;
-          const unsigned id = (unsigned)(i + head);
-          const bool hit = here && takes(value, id);
-          const unsigned hits = __ballot_sync(0xffffffffu, hit);
-          if (hits) {
-            int at = 0;
-            if (lane == 0) at = atomicAdd(&sh.n_keys, __popc(hits));
-            at = __shfl_sync(0xffffffffu, at, 0);
-            seen = at + __popc(hits);
-            at += __popc(hits & ((1u << lane) - 1u));
-            if (hit && at < KEY_CAP) sh.keys[at] = rank_key(value, id);
-          }
+      // Every column above `limit` becomes a key; returns how long the warp saw the list get.  A key that finds the list full is not
+      // written, and the length tells.
+      auto push = [&](float limit) {
+        if (__ballot_sync(0xffffffffu, !(cm <= limit)) == 0u) return 0;
+        unsigned hits = 0u;
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+          for (int e = 0; e < VN; ++e) hits |= Vec<T>::get(raw[j], e) > limit ? 1u << (j * VN + e) : 0u;
+        const int mine = __popc(hits);
+        int upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int t = __shfl_up_sync(0xffffffffu, upto, o);
+          if (lane >= o) upto += t;
+        }
+        int at = 0;
+        if (lane == 31) at = atomicAdd(&sh.n_keys, upto);
+        const int seen = __shfl_sync(0xffffffffu, at + upto, 31);
+        at = __shfl_sync(0xffffffffu, at, 31) + upto - mine;
+        while (hits) {
+          const int k = __ffs(hits) - 1;
+          hits &= hits - 1;
+          const unsigned id = (unsigned)((long)(c + k / VN * NT + tid) * VN + k % VN + head);
+          const u64 key = rank_key(pick<T, NV>(raw, k), id);
+          if (at < KEY_CAP) sh.keys[at] = key;
+          ++at;
         }
         return seen;
       };
       auto settle = [&](int n) {                              // after a prune
-        tau = n < top ? -INFINITY : rank_value(sh.keys[top - 1]);
-        open = n < top || tau != tau;                         // (NaN is the least there is: everything comes before it)
+        if (n >= top) tau = rank_value(sh.keys[top - 1]);
         __syncthreads();
       };
-      int seen = 0;
-      if (!open) seen = push(__ballot_sync(0xffffffffu, !(cm <= tau)), [&](float v, unsigned) { return v > tau; });
-      if (__syncthreads_or(open || seen > LONG_LIST)) {
+      float limit = tau;
+      bool bounded = false;
+      if (c == v_begin) {
+        limit = nextafterf(warp_bound(cm == cm ? cm : -INFINITY, top, sh), -INFINITY);
+        bounded = true;
+      }
+      for (;;) {
+        const int seen = push(limit);
+        if (!__syncthreads_or(c == v_begin || seen > long_list)) break;
         int n = sh.n_keys;
-        const bool full = n > KEY_CAP;
         __syncthreads();
-        if (!open && !full) {
-          settle(prune(n, top, sh));
-        } else {
-          // The first chunk, or one that brought more than the list holds: cut it by its own bound.  Keys of this chunk that are in the
-          // list already go first.
-          const unsigned id0 = (unsigned)(c * (long)VN + head), id1 = (unsigned)(min(v_end, c + STEP) * (long)VN + head);
-          auto older = [&](u64 key) { return (unsigned)rank_id(key) < id0 || (unsigned)rank_id(key) >= id1; };
-          if (full) {
-            n = compact(KEY_CAP, sh, older);
-            if (n >= top) settle(prune(n, top, sh));
-          }
-          int e_best = -1;                                    // the first of the thread's columns that is its maximum
-#pragma unroll
-          for (int j = NV - 1; j >= 0; --j)
-#pragma unroll
-            for (int e = VN - 1; e >= 0; --e)
-              if (Vec<T>::get(raw[j], e) == cm) e_best = j * VN + e;
-          const int v_best = c + e_best / VN * NT + tid;
-          u64 best = 0ull;
-          if (e_best >= 0 && v_best < v_end && (open || cm > tau)) best = rank_key(cm, (unsigned)((long)v_best * VN + e_best % VN + head));
-          const u64 bound = warp_bound(best, top, sh);
-          const bool was_open = open;
-          const float was_tau = tau;
-          auto takes = [&](float v, unsigned id) { return (was_open || v > was_tau) && rank_key(v, id) >= bound; };
-          push(__ballot_sync(0xffffffffu, bound == 0ull || best >= bound || cm != cm), takes);      // (NaN hides a thread's maximum)
+        if (n <= KEY_CAP) {
+          if (n >= top && c + STEP < v_end) settle(prune(n, top, sh));
+          break;
+        }
+        // More than the list holds: the chunk's keys that are in it go, and the chunk comes again, cut by its own bound.
+        const unsigned id0 = (unsigned)(c * (long)VN + head), id1 = (unsigned)(min(v_end, c + STEP) * (long)VN + head);
+        n = compact(KEY_CAP, -INFINITY, id0, id1, sh);
+        if (n >= top) settle(prune(n, top, sh));
+        if (!bounded) {
+          limit = fmaxf(tau, nextafterf(warp_bound(cm == cm ? cm : -INFINITY, top, sh), -INFINITY));
+          bounded = true;
+          continue;
+        }
+        // Still too many (one value in most places, or most of them masked): one vector of each thread at a time.
+#pragma unroll 1
+        for (int j = 0; j < NV; ++j) {
+          const int v = c + j * NT + tid;
+          if (v < v_end)
+#pragma unroll 1
+            for (int e = 0; e < VN; ++e) {
+              const long i = (long)v * VN + e;
+              const float value = kf_load(body, i);
+              if (value > tau) sh.keys[atomicAdd(&sh.n_keys, 1)] = rank_key(value, (unsigned)(i + head));
+            }
           __syncthreads();
           n = sh.n_keys;
           __syncthreads();
-          if (n <= KEY_CAP) {
-            if (bound != 0ull) {                              // at least `top` columns reach it
-              tau = rank_value(bound);
-              open = false;
-            } else if (n >= top) {
-              settle(prune(n, top, sh));
-            }
-          } else {                                            // still too many (a chunk full of NaN): one vector of each thread at a time
-            n = compact(KEY_CAP, sh, older);
-#pragma unroll 1
-            for (int j = 0; j < NV; ++j) {
-              const int v = c + j * NT + tid;
-              if (v < v_end)
-#pragma unroll 1
-                for (int e = 0; e < VN; ++e) {
-                  const long i = (long)v * VN + e;
-                  const float value = kf_load(body, i);
-                  if (open || value > tau) sh.keys[atomicAdd(&sh.n_keys, 1)] = rank_key(value, (unsigned)(i + head));
-                }
-              __syncthreads();
-              n = sh.n_keys;
-              __syncthreads();
-              settle(prune(n, top, sh));
-            }
-          }
+          settle(prune(n, top, sh));
         }
+        break;
       }
     }
 #pragma unroll
@@ -427,10 +465,34 @@ token_logprobs_kernel(const T* __restrict__ logits, long ld, int V, const int* _
       before += all.before[r];
     }
     if (TOP) {
-      for (int i = tid; i < slices * top; i += NT) sh.keys[i] = all.keys[i];
+      // The lists are in order: at least `top` of their keys reach the smallest of the lists' q-th keys, q = ceil(top / slices).
+      const int q = (top + slices - 1) / slices;
+      u64 bound = all.keys[q - 1];
+      for (int r = 1; r < slices; ++r) bound = min(bound, all.keys[r * top + q - 1]);
+      if (tid == 0) sh.n_keys = 0;
       __syncthreads();
-      prune(slices * top, top, sh);
+      for (int i = tid; i < slices * top; i += NT) {
+        const u64 key = all.keys[i];
+        if (key != 0ull && key >= bound) sh.keys[atomicAdd(&sh.n_keys, 1)] = key;
+      }
+      __syncthreads();
+      n = sh.n_keys;
+      rank_keys(sh.keys, n, top, sh);
     }
+  }
+  if (TOP && n < top) {
+    // Fewer columns above -inf than alternatives: the first masked ones follow, then NaN, each in order of their ids.
+    if (warp == 0)
+      for (int kind = 0; kind < 2; ++kind)
+        for (int i0 = 0; i0 < V && n < top; i0 += 32) {
+          const float v = i0 + lane < V ? kf_load(x, i0 + lane) : 0.f;
+          const bool hit = i0 + lane < V && (kind == 0 ? v == -INFINITY : v != v);
+          const unsigned hits = __ballot_sync(0xffffffffu, hit);
+          const int at = n + __popc(hits & ((1u << lane) - 1u));
+          if (hit && at < top) sh.sorted[at] = rank_key(v, (unsigned)(i0 + lane));
+          n += __popc(hits);
+        }
+    __syncthreads();
   }
   if (st.m == INFINITY) st.m = __int_as_float(0x7fffffff);
   const bool empty = st.m == -INFINITY;
@@ -505,10 +567,12 @@ KF_API int kf_token_logprobs(const void* logits, int dt, long ld, int R, int V, 
   if (R <= 0) return KF_OK;
   if (V <= 0 || V > 0x7fffff00 || R > (1 << 27) || top < 0 || top > TOP_MAX || top > V || (!tokens && (logprob || rank))) return KF_ERR_SIZE;
   if (((uintptr_t)logits & (dt == KF_F32 ? 3 : 1)) != 0) return KF_ERR_ALIGN;
-  // Blocks for every SM twice over, but no slice below a chunk.
+  // A row is cut while its slices still fit the device at once (two blocks an SM) and none falls below a chunk.  32-bit logits, L2
+  // flushed, slices 1 / 2 / 4 / 8 / 16: 64 x 256,000 with 20 alternatives 49 / 35 / 31 / 39 / 56 us, 8 x 256,000 47 / 32 / 23 / 18 / 18,
+  // 512 x 256,000 132 / 139 / 174 / 228 / 339, 301 x 32,003 28 / 35 / 43 / 74 / 142.
   const int chunks = kf_ceil_div(V, CHUNK);
   int slices = 1;
-  while (slices < MAX_SLICES && slices < chunks && (long)R * slices < 2l * kf_sm_count()) slices *= 2;
+  while (slices < MAX_SLICES && slices < chunks && (long)R * slices <= kf_sm_count()) slices *= 2;
 #ifdef KF_TUNING
   if (g_slices > 0) slices = g_slices;
 #endif
