@@ -15,9 +15,11 @@
 // column must exceed to join them.  The first chunk is cut by a bound that at least k of its columns reach (`warp_bound`) and
 // leaves the exact k-th value as tau.  From then on a column costs one comparison (of the thread's maximum), and a random row
 // brings k * 8,192 / (columns seen) keys a chunk; a list grown long is pruned to its k best, which raises tau.
-#include "common.cuh"
+#include "row_stats.cuh"
 
 namespace {
+
+using namespace kf_row;
 
 constexpr int TOP_MAX = 64;
 constexpr int NT = 256, WARPS = NT / 32;
@@ -26,9 +28,6 @@ constexpr int CHUNK = NT * PER_THREAD;
 constexpr int MAX_SLICES = 16;
 constexpr int KEY_CAP = NT * 8 + TOP_MAX;                    // keys held at most: a vector of every thread beside the k best
 constexpr int FEW_KEYS = 256;                                // up to here keys are ranked by counting the larger ones at once
-constexpr float LOG2E = 1.4426950408889634f;
-
-typedef unsigned long long u64;
 
 __device__ __forceinline__ unsigned orderable(float v) {     // larger float <=> larger unsigned; -0 as +0; NaN below everything
   const unsigned b = __float_as_uint(v == 0.f ? 0.f : v);
@@ -41,44 +40,6 @@ __device__ __forceinline__ float rank_value(u64 key) {
   return o == 0u ? __int_as_float(0x7fffffff) : __uint_as_float((o & 0x80000000u) ? (o & 0x7FFFFFFFu) : ~o);
 }
 __device__ __forceinline__ int rank_id(u64 key) { return (int)(0xFFFFFFFFu - (unsigned)key); }
-
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float exp2_fast(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-
-// Two 32-bit numbers in one instruction each (sm_100a)
-__device__ __forceinline__ u64 pack2(float a, float b) {
-  u64 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float2 unpack2(u64 v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ u64 add2(u64 a, u64 b) {
-  u64 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ u64 mul2(u64 a, u64 b) {
-  u64 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ u64 fma2(u64 a, u64 b, u64 c) {
-  u64 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
 
 // Sixteen bytes of a row as floats
 template <typename T> struct Vec;
@@ -114,24 +75,6 @@ __device__ __forceinline__ float pick(const uint4 (&raw)[NV], int at) {
     word >>= 1;
   }
   return Vec<T>::half_of(w[0], at);
-}
-
-// Running maximum, sum of exponentials and sum of d exp(d), and how a second set joins the first.
-struct Stats { float m, s, u; };
-__device__ __forceinline__ void move_to(Stats& a, float m) {
-  if (m != a.m) {
-    const float d = a.m - m, f = exp2_fast(d * LOG2E);
-    a.u = a.s == 0.f ? 0.f : f * (a.u + d * a.s);
-    a.s *= f;
-    a.m = m;
-  }
-}
-__device__ __forceinline__ void join(Stats& a, Stats b) {
-  const float m = max_nan(a.m, b.m);
-  move_to(a, m);
-  move_to(b, m);
-  a.s += b.s;
-  a.u += b.u;
 }
 
 struct Shared {
@@ -290,25 +233,7 @@ token_logprobs_kernel(const T* __restrict__ logits, long ld, int V, const int* _
 #pragma unroll
       for (int e = 0; e < VN; ++e) cm = max_nan(cm, Vec<T>::get(raw[j], e));
     move_to(st, max_nan(st.m, cm));
-    {
-      const float ref = st.m == -INFINITY ? 0.f : st.m;
-      const u64 minus = pack2(-ref, -ref), scale = pack2(LOG2E, LOG2E);
-      u64 s2 = 0ull, u2 = 0ull;
-#pragma unroll
-      for (int j = 0; j < NV; ++j)
-#pragma unroll
-        for (int e = 0; e < VN; e += 2) {
-          float2 d = unpack2(add2(pack2(Vec<T>::get(raw[j], e), Vec<T>::get(raw[j], e + 1)), minus));
-          const u64 low = pack2(fmaxf(d.x, -200.f), fmaxf(d.y, -200.f));    // exp(-200) is 0 in 32 bits, and 0 * -200 is 0
-          d = unpack2(mul2(low, scale));
-          const u64 w = pack2(exp2_fast(d.x), exp2_fast(d.y));
-          s2 = add2(s2, w);
-          u2 = fma2(low, w, u2);
-        }
-      const float2 s = unpack2(s2), u = unpack2(u2);
-      st.s += s.x + s.y;
-      st.u += u.x + u.y;
-    }
+    add_exponentials<PER_THREAD>(st, [&](int i) { return Vec<T>::get(raw[i / VN], i % VN); });
     if (RANK) {
       // Columns before the token count when they equal it, columns behind it do not: they must exceed the next lower number, or the
       // token's own.  One by one where the chunk holds the token, ends early (its masked places are no columns) or the token is masked.
@@ -494,19 +419,15 @@ token_logprobs_kernel(const T* __restrict__ logits, long ld, int V, const int* _
         }
     __syncthreads();
   }
-  if (st.m == INFINITY) st.m = __int_as_float(0x7fffffff);
-  const bool empty = st.m == -INFINITY;
-  const float log_s = logf(st.s);
   if (tid == 0) {
-    if (logprob) logprob[row] = !inside ? __int_as_float(0x7fffffff) : (empty ? -INFINITY : (given - st.m) - log_s);
-    if (entropy) entropy[row] = empty ? 0.f : log_s - st.u / st.s;
+    if (logprob) logprob[row] = row_logprob(st, inside ? given : __int_as_float(0x7fffffff));
+    if (entropy) entropy[row] = row_entropy(st);
     if (RANK) rank_out[row] = inside ? before : -1;
   }
   if (TOP && tid < top) {
     const u64 key = sh.sorted[tid];
-    const float v = rank_value(key);
     if (top_ids) top_ids[(size_t)row * top + tid] = rank_id(key);
-    if (top_logprobs) top_logprobs[(size_t)row * top + tid] = (empty && v == v) ? -INFINITY : (v - st.m) - log_s;
+    if (top_logprobs) top_logprobs[(size_t)row * top + tid] = row_logprob(st, rank_value(key));
   }
 }
 

@@ -47,6 +47,7 @@ def library():
                 path = _build.build()
                 lib = ctypes.CDLL(path)
                 lib.kf_last_cuda_error.restype = ctypes.c_char_p
+                lib.kf_head_logprobs_workspace.restype = ctypes.c_long
                 # kernels may start before their predecessor in the stream has finished (each waits for it before
                 # touching dependent memory); KUNGFU_PDL=0 switches that off
                 lib.kf_set_pdl(0 if os.environ.get("KUNGFU_PDL", "1") == "0" else 1)
@@ -351,7 +352,7 @@ def raise_on_device_error(device=None) -> None:
     code = device_error(device)
     if code:
         where, what = divmod(code, 16)
-        kernel = {0: "a product", 1: "prompt attention", 3: "a mixture's experts"}.get(where, "unknown")
+        kernel = {0: "a product", 1: "prompt attention", 3: "a mixture's experts", 4: "the head's log probabilities"}.get(where, "unknown")
         kinds = ("a stage was never freed", "operands never arrived", "scores or sums never came") if where == 1 else (
             "operands never arrived", "a stage was never freed", "an accumulator was never completed")
         raise KernelError(f"a kernel gave up waiting (code {code}, the first to give up: {kernel}, "
@@ -1501,6 +1502,16 @@ def head_logprobs(x, weight, tokens, out_logprob, *, out_entropy=None, softcap: 
         return
     if not x.is_cuda:
         _p(x)
+    lib = library()
+    if use_tensor_cores and x.dtype == torch.bfloat16 and weight.dtype == torch.bfloat16:
+        if lib.kf_head_logprobs_supported(_p(x), _p(weight), K):
+            # its own workspace for every call: calls on several streams, and graphs replayed at a time, do not share sums
+            work = torch.empty(lib.kf_head_logprobs_workspace(R, V), dtype=torch.float32, device=x.device)
+            _check(lib.kf_head_logprobs(_p(x), _p(weight), _p(tokens), R, V, K, _f(softcap), _p(out_logprob), _p(out_entropy), _p(work),
+                                        _p(_dev_scratch(x.device)["error"]), _stream()), what)
+            add_launches(1)
+            return
+        note_fallback(f"{what}: rows of {K} bfloat16 elements are no multiple of 16 bytes (or a base is unaligned)")
     step = max(1, min(R, LOGITS_PIECE_BYTES // (4 * V)))
     logits = torch.empty((step, V), dtype=torch.float32, device=x.device)
     for a in range(0, R, step):

@@ -161,3 +161,32 @@ def test_streams_and_graphs():
         torch.cuda.synchronize()
         assert all(torch.equal(lp, w[0]) for lp, w in zip(outs, want))
     ops.raise_on_device_error()
+
+
+# pairs and single blocks; the loads stop before the first stage, inside the first run of K and beyond the ring
+@pytest.mark.parametrize("R", [20, 300])
+@pytest.mark.parametrize("drop", [0, 3, 9])
+def test_a_product_whose_operands_never_arrive(R, drop):
+    """A test hook makes the producers leave out their loads from a stage on, with a limit of 2 ms: the kernel comes back by itself with its
+    code and NaN, and is right again after."""
+    import ctypes
+    from kungfu_b200 import ops
+    lib = ops.library()
+    x, w, t = make(R, 1024, 3000, torch.bfloat16)
+    right = run(x, w, t, 0.0)
+    torch.cuda.synchronize()
+    assert ops.device_error() == 0
+    assert lib.kf_test_head_give_up(ctypes.c_ulonglong(2_000_000), drop) == 0
+    try:
+        lp, _ = run(x, w, t, 0.0)
+        torch.cuda.synchronize()
+        assert ops.device_error() == 65
+        with pytest.raises(ops.KernelError, match="the head's log probabilities, operands never arrived"):
+            ops.raise_on_device_error()
+        assert bool(torch.isnan(lp).all())
+    finally:
+        assert lib.kf_test_head_give_up(ctypes.c_ulonglong(0), -1) == 0
+        ops.clear_device_error()
+    again = run(x, w, t, 0.0)
+    ops.raise_on_device_error()
+    assert all(torch.equal(a, b) for a, b in zip(again, right))
