@@ -47,7 +47,13 @@ def library():
                 path = _build.build()
                 lib = ctypes.CDLL(path)
                 lib.kf_last_cuda_error.restype = ctypes.c_char_p
+                vp, ci = ctypes.c_void_p, ctypes.c_int
+                lib.kf_token_logprobs.argtypes = [vp, ci, ctypes.c_long, ci, ci, vp, vp, vp, vp, ci, vp, vp, vp]
+                lib.kf_head_logprobs.argtypes = [vp, vp, vp, ci, ci, ci, ctypes.c_float, vp, vp, vp, vp, vp]
+                lib.kf_head_logprobs_supported.argtypes = [vp, vp, ci]
+                lib.kf_head_logprobs_workspace.argtypes = [ci, ci]
                 lib.kf_head_logprobs_workspace.restype = ctypes.c_long
+                lib.kf_copy_pages.argtypes = [vp, vp, ci, vp, vp, ci, vp]
                 # kernels may start before their predecessor in the stream has finished (each waits for it before
                 # touching dependent memory); KUNGFU_PDL=0 switches that off
                 lib.kf_set_pdl(0 if os.environ.get("KUNGFU_PDL", "1") == "0" else 1)
@@ -1407,30 +1413,27 @@ def topk_lse(logits, k: int, out_ids, out_vals, out_lse) -> None:
 
 # ---- log probabilities and copies of pages ----------------------------------------------------------------------------
 
-def _same_device(what: str, *tensors) -> None:
-    """Every tensor of a call lives on one device, and that is the one launches go to."""
-    devices = {t.device for t in tensors if t is not None}
-    if len(devices) > 1:
-        raise KernelError(f"{what}: tensors on several devices ({', '.join(sorted(str(d) for d in devices))})")
-    for d in devices:
-        if d.type == "cuda" and d.index != torch.cuda.current_device():
-            raise KernelError(f"{what}: tensors on {d}, but the current device is cuda:{torch.cuda.current_device()}")
+def _checked(what: str, device: int, tensors) -> None:
+    """Each of (name, tensor or None, shape, element type) is contiguous, of that shape and type, and on that device."""
+    for name, t, shape, dtype in tensors:
+        if t is not None:
+            if t.shape != shape or t.dtype != dtype or not t.is_contiguous():
+                raise KernelError(f"{what}: {name} is {tuple(t.shape)} {t.dtype}, not contiguous {tuple(shape)} {dtype}")
+            if t.get_device() != device:
+                raise KernelError(f"{what}: {name} is on another device than the call's first tensor")
 
 
-def _check_out(what: str, name: str, t, shape: tuple, dtype: torch.dtype) -> None:
-    if t is not None and (tuple(t.shape) != shape or t.dtype != dtype or not t.is_contiguous()):
-        raise KernelError(f"{what}: {name} is {tuple(t.shape)} {t.dtype}, not contiguous {shape} {dtype}")
+def _current(what: str, device: int):
+    """The stream of a launch for tensors on `device` (its index; -1: none), which has to be the current device."""
+    if device < 0:
+        raise KernelError("kungfu_b200 kernels run on CUDA tensors only; there is no CPU path")
+    if device != torch._C._cuda_getDevice():
+        raise KernelError(f"{what}: tensors on cuda:{device}, but the current device is cuda:{torch.cuda.current_device()}")
+    return _pinned_stream if _pinned_stream is not None else torch._C._cuda_getCurrentRawStream(device)
 
 
-def _check_tokens(what: str, tokens, rows: int, logprob, rank=None) -> None:
-    if tokens is None:
-        if logprob is not None or rank is not None:
-            raise KernelError(f"{what}: log probabilities and ranks need the tokens they are of")
-        return
-    if tuple(tokens.shape) != (rows,) or tokens.dtype != torch.int32 or not tokens.is_contiguous():
-        raise KernelError(f"{what}: tokens are {tuple(tokens.shape)} {tokens.dtype}, not contiguous ({rows},) torch.int32")
-    _check_out(what, "out_logprob", logprob, (rows,), torch.float32)
-    _check_out(what, "out_rank", rank, (rows,), torch.int32)
+def _address(t):
+    return None if t is None else t.data_ptr()
 
 
 MAX_TOP_LOGPROBS = 64           # alternatives that `token_logprobs` ranks
@@ -1451,29 +1454,30 @@ def token_logprobs(logits, tokens, out_logprob, *, out_entropy=None, out_rank=No
     if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16):
         raise KernelError(f"{what}: logits are {tuple(logits.shape)} {logits.dtype}, not rows of float32 or bfloat16")
     R, V = logits.shape
-    if V < 1 or (V > 1 and logits.stride(1) != 1):
+    ld, step = logits.stride()
+    if V < 1 or (V > 1 and step != 1):
         raise KernelError(f"{what}: the columns of a row must lie side by side (strides {tuple(logits.stride())}, {V} columns)")
-    _check_tokens(what, tokens, R, out_logprob, out_rank)
-    _check_out(what, "out_entropy", out_entropy, (R,), torch.float32)
+    if tokens is None and (out_logprob is not None or out_rank is not None):
+        raise KernelError(f"{what}: log probabilities and ranks need the tokens they are of")
     top = 0
-    for name, t, dtype in (("out_top_ids", out_top_ids, torch.int32), ("out_top_logprobs", out_top_logprobs, torch.float32)):
+    for t in (out_top_ids, out_top_logprobs):
         if t is not None:
             k = t.shape[-1] if t.dim() else 0
             if not 1 <= k <= min(MAX_TOP_LOGPROBS, V) or (top and k != top):
                 raise KernelError(f"{what}: {k} alternatives are not 1..min({MAX_TOP_LOGPROBS}, {V}), or not the same in both outputs")
             top = k
-            _check_out(what, name, t, (R, k), dtype)
     if out_logprob is None and out_entropy is None and out_rank is None and top == 0:
         raise KernelError(f"{what}: nothing to compute")
-    outs = (out_logprob, out_entropy, out_rank, out_top_ids, out_top_logprobs)
-    _same_device(what, logits, tokens, *outs)
+    device = logits.get_device()
+    _checked(what, device, (("tokens", tokens, (R,), torch.int32), ("out_logprob", out_logprob, (R,), torch.float32),
+                            ("out_entropy", out_entropy, (R,), torch.float32), ("out_rank", out_rank, (R,), torch.int32),
+                            ("out_top_ids", out_top_ids, (R, top), torch.int32), ("out_top_logprobs", out_top_logprobs, (R, top), torch.float32)))
     if R == 0:
         return
-    if not logits.is_cuda:
-        _p(logits)                                          # refuses, with the reason
-    _check(library().kf_token_logprobs(ctypes.c_void_p(logits.data_ptr()), _dt(logits), ctypes.c_long(logits.stride(0)), R, V, _p(tokens),
-                                       _p(out_logprob), _p(out_entropy), _p(out_rank), top, _p(out_top_ids),
-                                       _p(out_top_logprobs), _stream()), what)
+    stream = _current(what, device)
+    _check(library().kf_token_logprobs(logits.data_ptr(), F32 if logits.dtype == torch.float32 else BF16, ld, R, V, _address(tokens),
+                                       _address(out_logprob), _address(out_entropy), _address(out_rank), top, _address(out_top_ids),
+                                       _address(out_top_logprobs), stream), what)
 
 
 LOGITS_PIECE_BYTES = 256 << 20  # logits held at a time where `head_logprobs` computes them first
@@ -1495,20 +1499,19 @@ def head_logprobs(x, weight, tokens, out_logprob, *, out_entropy=None, softcap: 
     (R, K), V = x.shape, weight.shape[0]
     if tokens is None or out_logprob is None:
         raise KernelError(f"{what}: tokens and out_logprob are needed")
-    _check_tokens(what, tokens, R, out_logprob)
-    _check_out(what, "out_entropy", out_entropy, (R,), torch.float32)
-    _same_device(what, x, weight, tokens, out_logprob, out_entropy)
+    device = x.get_device()
+    _checked(what, device, (("weight", weight, (V, K), weight.dtype), ("tokens", tokens, (R,), torch.int32),
+                            ("out_logprob", out_logprob, (R,), torch.float32), ("out_entropy", out_entropy, (R,), torch.float32)))
     if R == 0:
         return
-    if not x.is_cuda:
-        _p(x)
-    lib = library()
+    stream = _current(what, device)
     if use_tensor_cores and x.dtype == torch.bfloat16 and weight.dtype == torch.bfloat16:
-        if lib.kf_head_logprobs_supported(_p(x), _p(weight), K):
+        lib = library()
+        if lib.kf_head_logprobs_supported(x.data_ptr(), weight.data_ptr(), K):
             # its own workspace for every call: calls on several streams, and graphs replayed at a time, do not share sums
             work = torch.empty(lib.kf_head_logprobs_workspace(R, V), dtype=torch.float32, device=x.device)
-            _check(lib.kf_head_logprobs(_p(x), _p(weight), _p(tokens), R, V, K, _f(softcap), _p(out_logprob), _p(out_entropy), _p(work),
-                                        _p(_dev_scratch(x.device)["error"]), _stream()), what)
+            _check(lib.kf_head_logprobs(x.data_ptr(), weight.data_ptr(), tokens.data_ptr(), R, V, K, softcap, out_logprob.data_ptr(),
+                                        _address(out_entropy), work.data_ptr(), _dev_scratch(x.device)["error"].data_ptr(), stream), what)
             add_launches(1)
             return
         note_fallback(f"{what}: rows of {K} bfloat16 elements are no multiple of 16 bytes (or a base is unaligned)")
@@ -1526,35 +1529,38 @@ def copy_pages(stores, src, dst) -> None:
     a copy of page src[i].  `src` and `dst` are host integers, as the cache manager's tables hold them.  No page may be named twice
     as a destination, or be both a source and a destination: the copies run at the same time."""
     what = "copy_pages"
-    stores = list(stores)
-    pairs = [(int(a), int(b)) for a, b in zip(src, dst)]
-    if len(pairs) != len(src) or len(pairs) != len(dst):
-        raise KernelError(f"{what}: {len(src)} sources for {len(dst)} destinations")
-    to = {b for _, b in pairs}
-    if len(to) != len(pairs) or any(a in to for a, _ in pairs):
+    stores, src, dst = list(stores), [int(i) for i in src], [int(i) for i in dst]
+    n = len(src)
+    if n != len(dst):
+        raise KernelError(f"{what}: {n} sources for {len(dst)} destinations")
+    to = set(dst)
+    if len(to) != n or not to.isdisjoint(src):
         raise KernelError(f"{what}: a page is a destination twice, or a source and a destination")
-    last = max((max(p) for p in pairs), default=-1)
-    if pairs and min(min(p) for p in pairs) < 0:
+    last = max(max(src), max(dst)) if n else -1
+    if n and min(min(src), min(dst)) < 0:
         raise KernelError(f"{what}: a page below 0")
+    device, bases, sizes = (stores[0].get_device() if stores else -1), [], []
     for t in stores:
-        if t.dim() < 1 or not t.is_contiguous() or t.shape[0] <= last:
+        shape = t.shape
+        if not shape or shape[0] <= last or not t.is_contiguous():
             raise KernelError(f"{what}: a store is contiguous and has more than {last} pages (got {tuple(t.shape)}, strides {tuple(t.stride())})")
-    _same_device(what, *stores)
-    live = [t for t in stores if t.numel()]
-    if not pairs or not live:
+        if t.get_device() != device:
+            raise KernelError(f"{what}: stores on several devices")
+        size = t.nbytes
+        if size:
+            bases.append(t.data_ptr())
+            sizes.append(size // shape[0])
+    if n == 0 or not bases:
         return
-    if not live[0].is_cuda:
-        _p(live[0])
+    stream = _current(what, device)
     lib = library()
-    for a in range(0, len(live), 64):
-        some = live[a:a + 64]
-        bases = (ctypes.c_int64 * len(some))(*[t.data_ptr() for t in some])
-        sizes = (ctypes.c_int64 * len(some))(*[t.numel() // t.shape[0] * t.element_size() for t in some])
-        for i in range(0, len(pairs), 256):
-            part = pairs[i:i + 256]
-            ids = (ctypes.c_int * len(part))
-            _check(lib.kf_copy_pages(bases, sizes, len(some), ids(*[p[0] for p in part]), ids(*[p[1] for p in part]), len(part),
-                                     _stream()), what)
+    for a in range(0, len(bases), 64):
+        m = min(64, len(bases) - a)
+        at, of = (ctypes.c_int64 * m)(*bases[a:a + m]), (ctypes.c_int64 * m)(*sizes[a:a + m])
+        for i in range(0, n, 256):
+            k = min(256, n - i)
+            ids = ctypes.c_int * k
+            _check(lib.kf_copy_pages(at, of, m, ids(*src[i:i + k]), ids(*dst[i:i + k]), k, stream), what)
 
 
 def device_arch() -> int:
