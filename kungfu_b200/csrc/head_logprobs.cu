@@ -25,10 +25,13 @@ using kf_row::Stats;
 using kf_row::u64;
 
 constexpr int BN = 256;                                         // vocabulary rows of a tile
-constexpr int RUN = 8;                                          // stages (of 64) of a run of K
+constexpr int RUN = 12, RUN_ALONE = 8;                          // most stages (of 64) of a run of K; of a K that is not cut
 constexpr int EPI_WARPS = 8, HEAD_THREADS = 64 + 32 * EPI_WARPS;
 constexpr int COLS = BN / 2;                                    // columns of a thread: two warps share 32 lanes
 constexpr int ERR_BASE = 64;
+// Blocks of 64 of K that arrive, are multiplied and are given back at a time.  Two for pairs, which the tensor cores bound (2,048 x 256,000 x
+// 2304 1,754 -> 1,570 us, 512 rows 437 -> 406); one for single blocks, which memory bounds (40 rows 210 us, two blocks 212).
+template <bool PAIR> constexpr int STAGE_BLOCKS = PAIR ? 2 : 1;
 
 // A test can make the producers leave out the loads of every stage from this one on (-1: never); see kf_test_head_give_up.
 static __device__ int g_test_drop_from_stage = -1;
@@ -52,6 +55,37 @@ __device__ __forceinline__ uint32_t in_leader(uint32_t addr) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
   return r;
 }
+// 32 columns of this thread's lane, on their way; after `tmem_arrived`, `after_wait16` keeps their uses behind the wait
+__device__ __forceinline__ void tmem_ld32_async(uint32_t taddr, float* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,"
+      "%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]),
+        "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]),
+        "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]),
+        "=f"(v[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_arrived() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void after_wait16(float* v) {
+  asm volatile("" : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]), "+f"(v[9]),
+               "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15])::"memory");
+}
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+// 1 / d for d in [1, 2^41], two at a time on the FMA units (the hardware's reciprocal shares its unit with the exponential, which bounds
+// the epilogue): a first guess from the bits, within 6 %, and three Newton steps r (2 - d r), each of which squares the error.
+__device__ __forceinline__ u64 reciprocal2(u64 d) {
+  const float2 f = kf_row::unpack2(d);
+  u64 r = kf_row::pack2(__int_as_float(0x7ef311c3 - __float_as_int(f.x)), __int_as_float(0x7ef311c3 - __float_as_int(f.y)));
+  const u64 minus = kf_row::pack2(-f.x, -f.y), two = kf_row::pack2(2.f, 2.f);
+#pragma unroll
+  for (int i = 0; i < 3; ++i) r = kf_row::mul2(r, kf_row::fma2(minus, r, two));
+  return r;
+}
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -60,7 +94,8 @@ __device__ __forceinline__ void cluster_sync() {
 template <bool PAIR>
 __global__ void __launch_bounds__(HEAD_THREADS, 1)
 head_logprobs_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ HeadArgs p) {
-  constexpr int A_BYTES = BM * BK * 2, B_ROWS = PAIR ? BN / 2 : BN, B_BYTES = B_ROWS * BK * 2, STAGE = A_BYTES + B_BYTES;
+  // KS blocks of 64 of K a stage, each a pair of operand tiles
+  constexpr int A_BYTES = BM * BK * 2, B_ROWS = PAIR ? BN / 2 : BN, B_BYTES = B_ROWS * BK * 2, KS = STAGE_BLOCKS<PAIR>, STAGE = KS * (A_BYTES + B_BYTES);
   constexpr int TMEM_COLS = 512;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -78,7 +113,8 @@ head_logprobs_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
   constexpr int TILE_ROWS = PAIR ? 2 * BM : BM;
   const int n_tt = (p.R + TILE_ROWS - 1) / TILE_ROWS, n_vt = (p.V + BN - 1) / BN;
   const long n_tiles = (long)n_vt * n_tt;
-  const int nkb = (p.K + BK - 1) / BK, runs = (nkb + RUN - 1) / RUN;
+  const int nkb = (p.K + KS * BK - 1) / (KS * BK);               // stages a tile: a last one that K does not fill multiplies zeros
+  const int runs = nkb * KS <= RUN_ALONE ? 1 : nkb * KS <= 2 * RUN ? 2 : (nkb * KS + RUN - 1) / RUN;
   const int per_run = (nkb + runs - 1) / runs;                    // runs of nearly equal length; (runs - 1) * per_run < nkb
   const int drop = g_test_drop_from_stage;
 
@@ -109,7 +145,7 @@ head_logprobs_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
   if (warp == 0) {
     // ---- TMA producer: the block's own tokens, its share of the vocabulary rows; a pair's bytes are counted in the leader --------
     if (lane == 0) {
-      const int bytes = p.x_rows * BK * 2 + B_BYTES;
+      const int bytes = KS * (p.x_rows * BK * 2 + B_BYTES);
       const uint32_t full0 = PAIR ? in_leader(smem_u32(&full[0])) : 0u;
       int s = 0, issued = 0;
       uint32_t ph = 1;
@@ -122,12 +158,16 @@ head_logprobs_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
           if (drop >= 0 && issued >= drop) { ok = false; break; }
           uint8_t* st = smem + (size_t)s * STAGE;
           if (rank == 0) mbar_expect_tx(&full[s], PAIR ? 2 * bytes : bytes);
-          if (PAIR) {
-            tma_load_pair(st, &tm_x, full0 + 8u * (uint32_t)s, kb * BK, t0);
-            tma_load_pair(st + A_BYTES, &tm_w, full0 + 8u * (uint32_t)s, kb * BK, v0);
-          } else {
-            tma_load_2d(st, &tm_x, &full[s], kb * BK, t0);
-            tma_load_2d(st + A_BYTES, &tm_w, &full[s], kb * BK, v0);
+#pragma unroll
+          for (int i = 0; i < KS; ++i) {
+            const int k = (kb * KS + i) * BK;
+            if (PAIR) {
+              tma_load_pair(st + i * A_BYTES, &tm_x, full0 + 8u * (uint32_t)s, k, t0);
+              tma_load_pair(st + KS * A_BYTES + i * B_BYTES, &tm_w, full0 + 8u * (uint32_t)s, k, v0);
+            } else {
+              tma_load_2d(st + i * A_BYTES, &tm_x, &full[s], k, t0);
+              tma_load_2d(st + KS * A_BYTES + i * B_BYTES, &tm_w, &full[s], k, v0);
+            }
           }
           ++issued;
           if (++s == p.stages) { s = 0; ph ^= 1; }
@@ -142,7 +182,7 @@ head_logprobs_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
     // ---- MMA issuer (a pair's leader) --------------------------------------------------------------------------------------
     if (lane == 0 && rank == 0) {
       const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(TILE_ROWS >> 4) << 24);
-      const uint64_t da0 = umma_desc(smem), db0 = umma_desc(smem + A_BYTES);
+      const uint64_t da0 = umma_desc(smem), db0 = umma_desc(smem + KS * A_BYTES);
       int s = 0;
       uint32_t ph = 0;
       long unit = 0;                                              // runs so far
@@ -158,9 +198,10 @@ head_logprobs_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
             if (!mbar_wait(&full[s], ph)) { give_up(ERR_WAIT_FULL); ok = false; break; }
             const uint64_t so = (uint64_t)((uint32_t)s * (uint32_t)(STAGE >> 4));
 #pragma unroll
-            for (int k = 0; k < BK / UMMA_K; ++k) {
+            for (int k = 0; k < KS * (BK / UMMA_K); ++k) {
               const uint32_t accumulate = (kb > kb0 || k > 0) ? 1u : 0u;
-              const uint64_t da = da0 + so + 2 * k, db = db0 + so + 2 * k;
+              const int block = k / (BK / UMMA_K), in_block = 2 * (k % (BK / UMMA_K));
+              const uint64_t da = da0 + so + block * (A_BYTES >> 4) + in_block, db = db0 + so + block * (B_BYTES >> 4) + in_block;
               if (PAIR)
                 asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
                              ::"r"(acc), "l"(da), "l"(db), "r"(idesc), "r"(accumulate) : "memory");
@@ -208,8 +249,6 @@ head_logprobs_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
       const bool idle = tt * TILE_ROWS + in_tile - lane >= p.R;   // none of the warp's rows exists
       const int col0 = vt * BN + half * COLS;
       float acc[COLS];
-#pragma unroll
-      for (int j = 0; j < COLS; ++j) acc[j] = 0.f;
 #pragma unroll 1
       for (int r = 0; r < runs; ++r, ++unit) {
         const int buf = (int)(unit & 1);
@@ -231,28 +270,41 @@ head_logprobs_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
           release();
           continue;
         }
+        const uint32_t from = lane_addr + buf * BN;
+        if (r == 0) {                                             // straight into the sums' registers, with one wait
 #pragma unroll
-        for (int q = 0; q < COLS; q += 16) {
-          float v[16];
-          tmem_ld16(lane_addr + buf * BN + q, v);
-          if (q + 16 == COLS) release();
+          for (int q = 0; q < COLS; q += 32) tmem_ld32_async(from + q, acc + q);
+          tmem_arrived();
 #pragma unroll
-          for (int j = 0; j < 16; ++j) acc[q + j] += v[j];
+          for (int q = 0; q < COLS; q += 16) after_wait16(acc + q);
+        } else {
+#pragma unroll
+          for (int q = 0; q < COLS; q += 32) {
+            float v[32];
+            tmem_ld32_async(from + q, v);
+            tmem_arrived();
+            after_wait16(v);
+            after_wait16(v + 16);
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+              const float2 sum = kf_row::unpack2(kf_row::add2(kf_row::pack2(acc[q + j], acc[q + j + 1]), kf_row::pack2(v[j], v[j + 1])));
+              acc[q + j] = sum.x;
+              acc[q + j + 1] = sum.y;
+            }
+          }
         }
+        release();
       }
       if (!ok || idle) continue;
       if (p.cap > 0.f) {
-        // cap tanh(v / cap) = cap - 2 cap / (exp(2 v / cap) + 1): within 2e-7 of the cap
+        // cap tanh(v / cap) = cap - 2 cap / (exp(2 v / cap) + 1): within 2e-7 of the cap.  From 2^40 on the quotient is nothing.
         const u64 in = kf_row::pack2(2.f * kf_row::LOG2E / p.cap, 2.f * kf_row::LOG2E / p.cap), one = kf_row::pack2(1.f, 1.f);
         const u64 twice = kf_row::pack2(-2.f * p.cap, -2.f * p.cap), cap2 = kf_row::pack2(p.cap, p.cap);
 #pragma unroll
         for (int j = 0; j < COLS; j += 2) {
           float2 e = kf_row::unpack2(kf_row::mul2(kf_row::pack2(acc[j], acc[j + 1]), in));
-          e = kf_row::unpack2(kf_row::add2(kf_row::pack2(kf_row::exp2_fast(e.x), kf_row::exp2_fast(e.y)), one));
-          float rx, ry;
-          asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(rx) : "f"(e.x));
-          asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(ry) : "f"(e.y));
-          e = kf_row::unpack2(kf_row::fma2(kf_row::pack2(rx, ry), twice, cap2));
+          const u64 d = kf_row::add2(kf_row::pack2(kf_row::exp2_fast(min_nan(e.x, 40.f)), kf_row::exp2_fast(min_nan(e.y, 40.f))), one);
+          e = kf_row::unpack2(kf_row::fma2(reciprocal2(d), twice, cap2));
           acc[j] = e.x;
           acc[j + 1] = e.y;
         }
@@ -298,22 +350,28 @@ head_logprobs_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
   }
 }
 
-// Joins the parts of 32 rows: eight warps read every eighth part, neighbouring lanes neighbouring rows.
-__global__ void __launch_bounds__(256) head_join_kernel(const float4* stats, int parts, int rows_padded, const float* given, const int* tokens,
-                                                        int R, int V, float* logprob, float* entropy) {
+// Joins the parts of 8 rows: neighbouring lanes take neighbouring rows, and 32 groups of threads every 32nd part.
+constexpr int JOIN_ROWS = 8, JOIN_THREADS = 256, JOIN_GROUPS = JOIN_THREADS / JOIN_ROWS;
+__global__ void __launch_bounds__(JOIN_THREADS) head_join_kernel(const float4* stats, int parts, int rows_padded, const float* given,
+                                                                 const int* tokens, int R, int V, float* logprob, float* entropy) {
   kf_pdl_trigger();
   kf_pdl_wait();
-  __shared__ Stats part[8][32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.x * 32 + lane;
+  __shared__ Stats part[JOIN_THREADS / 32][JOIN_ROWS];
+  const int tid = threadIdx.x, row = blockIdx.x * JOIN_ROWS + tid % JOIN_ROWS;
   Stats st = {-INFINITY, 0.f, 0.f};
-  for (int i = warp; i < parts; i += 8) {
+#pragma unroll 8
+  for (int i = tid / JOIN_ROWS; i < parts; i += JOIN_GROUPS) {
     const float4 f = stats[(size_t)i * rows_padded + row];
     kf_row::join(st, {f.x, f.y, f.z});
   }
-  part[warp][lane] = st;
+#pragma unroll
+  for (int o = JOIN_ROWS; o < 32; o *= 2)
+    kf_row::join(st, {__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.s, o), __shfl_xor_sync(0xffffffffu, st.u, o)});
+  if (tid % 32 < JOIN_ROWS) part[tid / 32][tid % 32] = st;
   __syncthreads();
-  if (warp > 0 || row >= R) return;
-  for (int i = 1; i < 8; ++i) kf_row::join(st, part[i][lane]);
+  if (tid >= JOIN_ROWS || row >= R) return;
+#pragma unroll
+  for (int i = 1; i < JOIN_THREADS / 32; ++i) kf_row::join(st, part[i][tid]);
   const int token = tokens[row];
   if (token < 0) return;
   logprob[row] = kf_row::row_logprob(st, token < V ? given[row] : __int_as_float(0x7fffffff));
@@ -330,8 +388,8 @@ int workers(int R, int V) {
 
 template <bool PAIR>
 int launch(const CUtensorMap& tx, const CUtensorMap& tw, HeadArgs p, int n_workers, cudaStream_t stream) {
-  constexpr int STAGE = BM * BK * 2 + (PAIR ? BN / 2 : BN) * BK * 2;
-  p.stages = PAIR ? 6 : 4;                                        // 192 KB
+  constexpr int STAGE = STAGE_BLOCKS<PAIR> * (BM + (PAIR ? BN / 2 : BN)) * BK * 2;
+  p.stages = PAIR ? 3 : 4;                                        // 192 KB
   const size_t smem = (size_t)p.stages * STAGE + 1024 + 256;
   static bool configured[64] = {};                                // by device
   int dev = 0;
@@ -397,7 +455,7 @@ KF_API int kf_head_logprobs(const void* x, const void* w, const int* tokens, int
   if (!tensor_map(x, R, K, box, &tx) || !tensor_map(w, V, K, pair ? BN / 2 : BN, &tw)) return KF_ERR_SETUP;
   const int rc = pair ? launch<true>(tx, tw, p, n_workers, stream) : launch<false>(tx, tw, p, n_workers, stream);
   if (rc != KF_OK) return rc;
-  kf_launch(head_join_kernel, dim3(kf_ceil_div(R, 32)), dim3(256), 0, stream, (const float4*)p.stats, 2 * n_workers, p.rows_padded,
+  kf_launch(head_join_kernel, dim3(kf_ceil_div(R, JOIN_ROWS)), dim3(JOIN_THREADS), 0, stream, (const float4*)p.stats, 2 * n_workers, p.rows_padded,
             (const float*)p.given, tokens, R, V, logprob, entropy);
   KF_CHECK_LAUNCH();
   return KF_OK;

@@ -163,9 +163,10 @@ def test_streams_and_graphs():
     ops.raise_on_device_error()
 
 
-# pairs and single blocks; the loads stop before the first stage, inside the first run of K and beyond the ring
+# pairs and single blocks; the loads stop before the first stage, inside the first run of K and beyond the ring (a pair's only tile has
+# 1,024 / 128 = 8 stages)
 @pytest.mark.parametrize("R", [20, 300])
-@pytest.mark.parametrize("drop", [0, 3, 9])
+@pytest.mark.parametrize("drop", [0, 3, 6])
 def test_a_product_whose_operands_never_arrive(R, drop):
     """A test hook makes the producers leave out their loads from a stage on, with a limit of 2 ms: the kernel comes back by itself with its
     code and NaN, and is right again after."""
