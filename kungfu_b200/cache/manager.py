@@ -14,6 +14,9 @@ declaration-driven shape but stores tokens in fixed-size pages:
   position they hold is out of reach of any later query: a query at position p reads keys
   j >= p - window + 1, so after a step that leaves the request at length n the pages that end at or
   before n - window + 1 go back (in a group of chunks of C positions: at or before floor(n / C) * C);
+* a request can be forked: the new one shares the parent's full pages, which nobody writes to again (a page goes back to the
+  pool when the last table that names it lets go of it), and gets copies of the last, partly filled pages and of the
+  fixed-size states, all copied on the device by one launch per group and one for the states;
 * every live request also owns one state slot (an index into dense per-request state arrays) for
   mixers that keep a state of fixed size; it is zeroed at admission.
 
@@ -27,6 +30,7 @@ import ctypes
 import numpy as np
 import torch
 
+from .. import ops
 from ..parts.base import StateBundle
 from .kinds import FixedStateView, PagedKVView, flatten_need, kind_of, lifetime_chunked, lifetime_keep, lifetime_of, lifetime_window       # the views are re-exported from here
 
@@ -67,6 +71,7 @@ def host_library():
                             ("kf_cache_reserve", [ctypes.c_int]), ("kf_cache_commit", [ctypes.c_int]),
                             ("kf_cache_pages_needed", [ctypes.c_int, ctypes.c_void_p])):
             getattr(lib, name).argtypes = [ctypes.c_void_p, i64] + extra
+        lib.kf_cache_fork.argtypes = [ctypes.c_void_p, i64, i64, ctypes.c_void_p]
         lib.kf_cache_table.argtypes = [ctypes.c_void_p, ctypes.c_int, i64, ctypes.c_void_p, ctypes.c_int]
         lib.kf_step_layout.argtypes = [ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
                                        ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_void_p]
@@ -210,6 +215,9 @@ class CacheManager:
             if self._units[s]:
                 stores = [u[2] for u in self._units[s]]
                 self.storage[s] = stores if isinstance(whole, StateBundle) else stores[0]
+        # what a fork copies: the paged stores of every group, the fixed-size states
+        self._group_stores: list[list] = [[store for s in g.slots for _n, kind, store in self._units[s] if kind.paged] for g in self.groups]
+        self._fixed_stores: list = [store for units in self._units for _n, kind, store in units if not kind.paged]
         G = len(self.groups)
         windows = (ctypes.c_int * max(G, 1))(*[(-1 if g.window is None else int(lifetime_window(g.window))) for g in self.groups])
         sizes = (ctypes.c_int * max(G, 1))(*pool_sizes)
@@ -325,6 +333,55 @@ class CacheManager:
         if rc != _OK:
             raise CacheError(f"commit for {request!r} failed (code {rc})")
 
+    def fork(self, parent, child) -> None:
+        """`child` becomes a live request that holds what `parent` holds (see `fork_all`)."""
+        self.fork_all([(parent, child)])
+
+    def fork_all(self, pairs) -> None:
+        """For every (parent, child): the child becomes a live request with the parent's length, its full pages (shared),
+        copies of its last, partly filled pages and of its fixed-size states, in stream order after what wrote them.  All
+        forks or none: raises OutOfPages or CacheError (no state slot, a parent that is not live or has reserved tokens, a child
+        that is live) with everything as it was.  A parent may be named often, and is not one of the children."""
+        pairs = list(pairs)
+        children = {c for _, c in pairs}
+        if len(children) != len(pairs) or any(p in children for p, _ in pairs):
+            raise CacheError("fork: a child named twice, or a parent that is one of the children")
+        G = max(len(self.groups), 1)
+        copies = (ctypes.c_int * (3 * G))()
+        pages: dict = {}                              # group -> (sources, destinations)
+        slots: tuple = ([], [])
+        made = []
+        try:
+            for parent, child in pairs:
+                if child in self._key:
+                    raise CacheError(f"request {child!r} is already live")
+                key = self._next_key
+                n = self._lib.kf_cache_fork(self._h, self.key_of(parent), key, copies)
+                if n == -_E_OUT_OF_PAGES:
+                    raise OutOfPages(f"fork of {parent!r}: a group has no free page for its last, partly filled one")
+                if n == -_E_NO_SLOT:
+                    raise CacheError(f"more than {self.max_requests} live requests")
+                if n < 0:
+                    raise CacheError(f"fork of {parent!r} failed (code {-n}; tokens reserved and not committed?)")
+                self._next_key += 1
+                self._key[child] = key
+                made.append(child)
+                for i in range(n):
+                    g, src, dst = copies[3 * i:3 * i + 3]
+                    of = pages.setdefault(g, ([], []))
+                    of[0].append(src)
+                    of[1].append(dst)
+                slots[0].append(self.state_slot(parent))
+                slots[1].append(self.state_slot(child))
+            for g, (src, dst) in pages.items():
+                ops.copy_pages(self._group_stores[g], src, dst)
+            if self._fixed_stores:
+                ops.copy_pages(self._fixed_stores, *slots)
+        except BaseException:
+            for child in made:
+                self.release(child)
+            raise
+
     def release(self, request) -> None:
         """The request is finished (or preempted): everything it holds goes back."""
         rc = self._lib.kf_cache_release(self._h, self.key_of(request))
@@ -380,6 +437,6 @@ class CacheManager:
         return sum(store.numel() * store.element_size() for units in self._units for _n, _k, store in units)
 
     def check(self) -> None:
-        """Every page is either free or in exactly one table; raises CacheError otherwise."""
+        """Every page is either free or in as many tables as hold it; raises CacheError otherwise."""
         if self._lib.kf_cache_check(self._h) != _OK:
             raise CacheError("page accounting is inconsistent: a page is lost, held twice, or a table entry is stale")

@@ -3,8 +3,10 @@
 Subcommands and option names follow it where it has them:
   inspect <model> [--json]      what the folder is, its tensors and what each layer keeps       (:19,213-311)
   describe                      capabilities and parameters of this build as JSON               (:21,149-152)
-  generate --model --ids ...    complete a prompt given as token ids                            (:107-136,611-645)
-  score --model --ids --prefix  greedy prediction (or top-k ids) at every position              (:30-55,173-197)
+  generate --model --ids ...    complete a prompt given as token ids                            (:107-136,611-645);
+                                --beams: the best answers of a beam search, --logprobs: every token scored (both ours)
+  score --model --ids --prefix  greedy prediction (or top-k ids) at every position              (:30-55,173-197);
+                                --logprobs: log probabilities, entropies and perplexity of the ids themselves (ours)
   bench --model --pp --tg --reps  prompt and generation throughput                              (:82-105,544-608)
   random-weights                write a model folder from a config.json and a seed (ours; the reference has no such mode)
 There is no tokenizer here: prompts are token ids (`--ids`), and output is always ids.
@@ -173,9 +175,20 @@ def cmd_generate(args) -> int:
     if args.ids is None:
         raise SystemExit("error: this build has no tokenizer; give the prompt as --ids '[1, 2, 3]'")
     ids = json.loads(args.ids)
-    eng = _engine(args)
+    eng = _engine(args, parallel=max(1, args.beams))
+    if args.beams > 1:
+        found = eng.beam_search(ids, beams=args.beams, max_tokens=args.max_tokens, ignore_eos=args.ignore_eos)
+        print(json.dumps({"prompt": ids, "beams": [{"generated": b.tokens, "logprob": b.logprob, "finish": b.finish_reason} for b in found]}))
+        return 0
     sampling = Sampling(temperature=args.temperature, top_k=args.top_k, top_p=args.top_p, min_p=args.min_p,
                         repeat_penalty=args.repeat_penalty)
+    if args.logprobs is not None:
+        rid = eng.add_request(ids, sampling, max_tokens=args.max_tokens, ignore_eos=args.ignore_eos, seed=args.seed, logprobs=args.logprobs)
+        while not eng.idle:
+            eng.step()
+        req = eng.requests[rid]
+        print(json.dumps({"prompt": ids, "generated": req.output, "scores": [_score_fields(t) for t in req.scores]}))
+        return 0
     out = eng.generate([ids], sampling, max_tokens=args.max_tokens, ignore_eos=args.ignore_eos, seed=args.seed)[0]
     eos = set(getattr(eng.cfg, "eos_token_id", ()) or ())
     if out and out[-1] in eos and not args.ignore_eos and not args.emit_ids:
@@ -186,11 +199,25 @@ def cmd_generate(args) -> int:
 
 # ---- score --------------------------------------------------------------------------------------------------
 
+def _score_fields(t) -> dict:
+    """A TokenScore as JSON (the rank where one was asked for)."""
+    doc = {"token": t.token, "logprob": t.logprob, "entropy": t.entropy}
+    if t.rank is not None:
+        doc.update(rank=t.rank, top=[[i, lp] for i, lp in t.top])
+    return doc
+
+
 def cmd_score(args) -> int:
     import torch
     from .engine.step import StepEntry
     ids = json.loads(args.ids)
     eng = _engine(args)
+    if args.logprobs:
+        scores = eng.score([ids], top=args.topk)[0]
+        total = sum(t.logprob for t in scores)
+        print(json.dumps({"ids": ids, "logprob": total, "perplexity": math.exp(-total / max(len(scores), 1)),
+                          "scores": [_score_fields(t) for t in scores]}))
+        return 0
     runner = eng.runner
     prefix = len(ids) if args.prefix is None else max(1, min(args.prefix, len(ids)))
     runner.cache.add_request("score")
@@ -323,15 +350,18 @@ def main(argv=None) -> int:
     p.add_argument("--min-p", type=float, default=0.0)
     p.add_argument("--repeat-penalty", type=float, default=1.0)
     p.add_argument("--seed", type=int, default=42)
+    p.add_argument("--beams", type=int, default=1, help="more than one: a beam search of that many open answers (no sampling)")
+    p.add_argument("--logprobs", type=int, default=None, help="score every generated token, with that many alternatives")
     p.add_argument("--events", action="store_true", help="print `kungfu event=` lines on stderr")
     _common(p)
     p.set_defaults(fn=cmd_generate)
-    p = sub.add_parser("score", help="greedy prediction at every position of a token sequence")
+    p = sub.add_parser("score", help="greedy prediction (or the log probability) at every position of a token sequence")
     p.add_argument("--model", required=True)
     p.add_argument("--ids", required=True)
     p.add_argument("--prefix", type=int, default=None, help="tokens fed as one batch before the rest go one at a time")
     p.add_argument("--ignore-eos", action="store_true")
     p.add_argument("--topk", type=int, default=0)
+    p.add_argument("--logprobs", action="store_true", help="the tokens' log probabilities and entropies (with --topk: ranks and alternatives too)")
     _common(p)
     p.set_defaults(fn=cmd_score)
     p = sub.add_parser("bench", help="prompt and generation throughput")

@@ -22,7 +22,7 @@ namespace {
 struct Pool {
   int n = 0;
   std::vector<int> free_list;           // pop_back hands out low ids first
-  std::vector<char> held;
+  std::vector<int> held;                // how many block tables name the page (more than one after a fork)
   long n_taken = 0;                     // pages handed out so far (more than n: pages were used again)
   explicit Pool(int n_pages) : n(n_pages), held(n_pages, 0) {
     free_list.reserve(n_pages);
@@ -37,10 +37,10 @@ struct Pool {
     ++n_taken;
     return p;
   }
+  void share(int p) { ++held[p]; }      // one more block table names a held page
   bool give_back(int p) {
     if (p < 0 || p >= n || !held[p]) return false;
-    held[p] = 0;
-    free_list.push_back(p);
+    if (--held[p] == 0) free_list.push_back(p);
     return true;
   }
 };
@@ -84,7 +84,7 @@ KF_HOST_API void kf_pool_destroy(void* p) { delete (Pool*)p; }
 KF_HOST_API int kf_pool_take(void* p) { return ((Pool*)p)->take(); }
 KF_HOST_API int kf_pool_give_back(void* p, int page) { return ((Pool*)p)->give_back(page) ? OK : E_PAGE_NOT_HELD; }
 KF_HOST_API int kf_pool_n_free(void* p) { return ((Pool*)p)->n_free(); }
-KF_HOST_API int kf_pool_is_held(void* p, int page) { Pool* q = (Pool*)p; return page >= 0 && page < q->n && q->held[page]; }
+KF_HOST_API int kf_pool_is_held(void* p, int page) { Pool* q = (Pool*)p; return page >= 0 && page < q->n && q->held[page] > 0; }
 
 // ---- cache manager ---------------------------------------------------------------------------------------------------
 KF_HOST_API void* kf_cache_create(int n_groups, const int* windows, const int* n_pages, int page_size, int max_requests,
@@ -119,7 +119,7 @@ KF_HOST_API int kf_cache_state_slot(void* h, int64_t req) {
 KF_HOST_API int kf_cache_pool_n_free(void* h, int g) { return ((Cache*)h)->groups[g].pool.n_free(); }
 KF_HOST_API int kf_cache_pool_is_held(void* h, int g, int page) {
   Pool& p = ((Cache*)h)->groups[g].pool;
-  return page >= 0 && page < p.n && p.held[page];
+  return page >= 0 && page < p.n && p.held[page] > 0;
 }
 KF_HOST_API long kf_cache_pool_n_taken(void* h, int g) { return ((Cache*)h)->groups[g].pool.n_taken; }
 KF_HOST_API const int* kf_cache_mirror(void* h, int g) { return ((Cache*)h)->groups[g].mirror.data(); }
@@ -230,6 +230,44 @@ KF_HOST_API int kf_cache_commit(void* h, int64_t req, int n_new) {
   return OK;
 }
 
+// `child` becomes a request that holds what `parent` holds: the parent's full pages are shared (nothing is written to a page
+// that its request has filled), a last, partly filled page of a group is a page of its own, to be copied.  `copies` receives
+// (group, source, destination) for each of those, at most one per group.  Returns how many, or -(error code) with nothing
+// changed; a parent with tokens reserved but not committed is refused.
+KF_HOST_API int kf_cache_fork(void* h, int64_t parent, int64_t child, int* copies) {
+  Cache* c = (Cache*)h;
+  auto it = c->reqs.find(parent);
+  if (it == c->reqs.end()) return -E_NOT_LIVE;
+  if (c->reqs.count(child)) return -E_ALREADY_LIVE;
+  if (it->second.reserved != 0) return -E_COMMIT;
+  if (c->free_slots.empty()) return -E_NO_SLOT;
+  const Request from = it->second;                           // a copy: the map may move its elements
+  const int tail = from.length % c->page_size ? from.length / c->page_size : -1;      // index of the partly filled page
+  auto has_tail = [&](size_t g) { return tail >= 0 && tail < from.n_entries[g] && c->row((int)g, from.slot)[tail] >= 0; };
+  for (size_t g = 0; g < c->groups.size(); ++g)
+    if (has_tail(g) && c->groups[g].pool.n_free() < 1) return -E_OUT_OF_PAGES;
+  Request to = from;
+  to.slot = c->free_slots.back();
+  c->free_slots.pop_back();
+  int n = 0;
+  for (size_t g = 0; g < c->groups.size(); ++g) {
+    const int* src = c->row((int)g, from.slot);
+    int* dst = c->row((int)g, to.slot);
+    std::copy(src, src + c->width, dst);
+    for (int i = 0; i < from.n_entries[g]; ++i)
+      if (src[i] >= 0 && !(i == tail)) c->groups[g].pool.share(src[i]);
+    if (has_tail(g)) {
+      dst[tail] = c->groups[g].pool.take();
+      copies[3 * n] = (int)g;
+      copies[3 * n + 1] = src[tail];
+      copies[3 * n + 2] = dst[tail];
+      ++n;
+    }
+  }
+  c->reqs.emplace(child, std::move(to));
+  return n;
+}
+
 KF_HOST_API int kf_cache_release(void* h, int64_t req) {
   Cache* c = (Cache*)h;
   auto it = c->reqs.find(req);
@@ -258,13 +296,13 @@ KF_HOST_API int kf_cache_table(void* h, int g, int64_t req, int* out, int cap) {
   return n;
 }
 
-// every page is either free or in exactly one table: OK or E_INCONSISTENT
+// every page is either free or in as many tables as it is held by: OK or E_INCONSISTENT
 KF_HOST_API int kf_cache_check(void* h) {
   Cache* c = (Cache*)h;
   for (size_t g = 0; g < c->groups.size(); ++g) {
     Pool& pool = c->groups[g].pool;
-    std::vector<char> seen(pool.n, 0);
-    int n_seen = 0;
+    std::vector<int> seen(pool.n, 0), last(pool.n, -1);
+    int nth = 0;
     for (auto& kv : c->reqs) {
       const Request& r = kv.second;
       const int* row = c->row((int)g, r.slot);
@@ -272,14 +310,18 @@ KF_HOST_API int kf_cache_check(void* h) {
         const int p = row[i];
         if (i >= r.n_entries[g]) { if (p != -1) return E_INCONSISTENT; continue; }
         if (p < 0) continue;
-        if (p >= pool.n || seen[p] || !pool.held[p]) return E_INCONSISTENT;
-        seen[p] = 1;
-        ++n_seen;
+        if (p >= pool.n || last[p] == nth) return E_INCONSISTENT;      // (no request names a page twice)
+        last[p] = nth;
+        ++seen[p];
       }
+      ++nth;
     }
     int n_held = 0;
-    for (int p = 0; p < pool.n; ++p) n_held += pool.held[p];
-    if (n_held != n_seen || n_held + pool.n_free() != pool.n) return E_INCONSISTENT;
+    for (int p = 0; p < pool.n; ++p) {
+      if (seen[p] != pool.held[p]) return E_INCONSISTENT;
+      n_held += pool.held[p] > 0;
+    }
+    if (n_held + pool.n_free() != pool.n) return E_INCONSISTENT;
   }
   return OK;
 }

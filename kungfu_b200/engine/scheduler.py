@@ -41,12 +41,14 @@ class Request:
     eos: tuple = ()
     ignore_eos: bool = False
     seed: int = 42
+    logprobs: int | None = None        # not None: every produced token is scored, with that many alternatives
     # state
     status: str = WAITING
     output: list = field(default_factory=list)
     n_cached: int = 0                  # tokens of `tokens()` whose keys/values are in the cache
     finish_reason: str | None = None
     n_preempted: int = 0
+    scores: list = field(default_factory=list)      # one TokenScore per token of `output` (None for one that was not scored)
     sampler_epoch: int = -1            # the admission (count of preemptions) for which the device holds its sampler state
 
     def __post_init__(self):

@@ -19,6 +19,7 @@ import numpy as np
 import torch
 
 from ..cache.manager import CacheManager, OutOfPages
+from ..sampling.scores import ScoreRows, check_alternatives
 
 
 @dataclass
@@ -71,6 +72,7 @@ class StepContext:
     # writing call per cache slot, before any that only reads (`DecoderModel`): the call that moves a fixed state on finds it
     # as the step before left it, however early it looks.
     states_settled = True
+    score = None                                  # (tokens, ScoreRows): a step that scores the tokens at its wanted places
 
     def __init__(self, runner: "Runner"):
         self._runner = runner
@@ -113,6 +115,7 @@ class Runner:
         self.act_dtype = act_dtype
         self.device = torch.device(device)
         self.buffers = BufferPool(self.device)
+        self._score_buffers = BufferPool(self.device)     # apart: no captured graph points at them
         self.vocab = model.vocab
         self._staging: list = []                  # ring of (pinned host block, event of its last copy)
         self._staging_next = 0
@@ -292,15 +295,7 @@ class Runner:
         self.validate(entries)
         if feedback is not None and any(len(e.tokens) != 1 for e in entries):
             raise StepError("tokens can only be fed back on the device to a step of single tokens")
-        reserved = []
-        try:
-            for e in entries:
-                self.cache.reserve(e.request, len(e.tokens))
-                reserved.append(e)
-        except OutOfPages:
-            for e in reserved:
-                self.cache.cancel_reservation(e.request)
-            raise
+        self._reserve(entries)
         try:
             bucket = self._graph_bucket(entries, greedy)
             self.last_logit_index = self._logit_index(entries, bucket)
@@ -323,27 +318,92 @@ class Runner:
         self.steps_run += 1
         return (logits, picked) if greedy else logits
 
+    def _reserve(self, entries) -> None:
+        """The pages for every entry's tokens, or none at all (raises OutOfPages)."""
+        reserved = []
+        try:
+            for e in entries:
+                self.cache.reserve(e.request, len(e.tokens))
+                reserved.append(e)
+        except OutOfPages:
+            for e in reserved:
+                self.cache.cancel_reservation(e.request)
+            raise
+
+    def score(self, entries: Sequence[StepEntry], targets: Sequence[Sequence[int]], top: int = 0) -> ScoreRows:
+        """Run the tokens of `entries` as one batch, like `step`, and return what the model says at each wanted place about a token
+        given for it: `targets[i]` names one token for every place that entry i wants (a token of -1: nothing is computed for that
+        place).  `top`: that many alternatives per place.  The result lives in a buffer that the next call overwrites."""
+        entries = list(entries)
+        self.validate(entries)
+        top = check_alternatives(top, self.vocab)
+        if len(targets) != len(entries) or any(len(t) != len(e.want) for e, t in zip(entries, targets)):
+            raise StepError("targets name one token for every wanted place of every entry")
+        flat = [int(t) for ts in targets for t in ts]
+        if any(not (-1 <= t < self.vocab) for t in flat):
+            raise StepError(f"a target is outside the vocabulary of {self.vocab}")
+        if not entries or not flat:
+            raise StepError("a step that scores wants at least one place")
+        self._reserve(entries)
+        try:
+            ctx = self._fill(entries, None, None)
+            words = self._score_buffers.get("score_rows", (ScoreRows.words(len(flat), top),), torch.int32)
+            rows = ScoreRows(words, len(flat), top)
+            tokens = torch.tensor(flat, dtype=torch.int32).to(self.device)
+            ctx.score = (tokens, rows)
+            self._forward(ctx)
+        except BaseException:
+            for e in entries:
+                self.cache.cancel_reservation(e.request)
+            raise
+        for e in entries:
+            self.cache.commit(e.request, len(e.tokens))
+        self.steps_run += 1
+        return rows
+
+    def score_rows(self, logits: torch.Tensor, tokens: torch.Tensor, top: int) -> ScoreRows:
+        """What rows of logits that a step has left on the device say about `tokens` (on the device too)."""
+        from .. import ops
+        n = logits.shape[0]
+        words = self._score_buffers.get("score_rows", (ScoreRows.words(n, top),), torch.int32)
+        rows = ScoreRows(words, n, top)
+        ops.token_logprobs(logits, tokens, rows.logprob, out_entropy=rows.entropy, out_rank=rows.rank, out_top_ids=rows.ids,
+                           out_top_logprobs=rows.top_logprobs)
+        return rows
+
     def fetch_async(self, ids: torch.Tensor, n: int):
         """Start the copy of `ids[:n]` (token ids on the device) to pinned host memory, in stream order after the step
         that wrote them and before anything that overwrites them; returns a function that waits for the copy and gives
         the ids as a list."""
+        wait = self._fetch_words(ids[:n], "_fetch_ring")
+        return lambda: wait().tolist()
+
+    def _fetch_words(self, words: torch.Tensor, ring_name: str):
+        """Start the copy of 32-bit words to pinned host memory, in stream order; returns a function that waits for it and gives them as
+        an array.  At most three later copies of the ring may start before that function is called."""
+        n = words.numel()
         if self.device.type != "cuda":
-            vals = ids[:n].tolist()
-            return lambda: vals
-        ring = getattr(self, "_fetch_ring", None)
-        if ring is None or ring[0][0].numel() < n:
+            held = words.clone().numpy()
+            return lambda: held
+        ring = getattr(self, ring_name, None)
+        if ring is None or ring["slots"][0][0].numel() < n:
             cap = max(64, 1 << (max(n, 1) - 1).bit_length())
-            ring = self._fetch_ring = [[torch.empty(cap, dtype=torch.int32, pin_memory=True), torch.cuda.Event()] for _ in range(4)]
-            self._fetch_next = 0
-        buf, ev = ring[self._fetch_next]
-        self._fetch_next = (self._fetch_next + 1) % len(ring)
-        buf[:n].copy_(ids[:n], non_blocking=True)
+            ring = {"slots": [[torch.empty(cap, dtype=torch.int32, pin_memory=True), torch.cuda.Event()] for _ in range(4)], "next": 0}
+            setattr(self, ring_name, ring)
+        buf, ev = ring["slots"][ring["next"]]
+        ring["next"] = (ring["next"] + 1) % len(ring["slots"])
+        buf[:n].copy_(words, non_blocking=True)
         ev.record()
 
         def wait():
             ev.synchronize()
-            return buf[:n].tolist()
+            return buf[:n].numpy()
         return wait
+
+    def fetch_scores(self, rows: ScoreRows):
+        """The same for the words of `rows`: a function that gives them as an array of its own."""
+        wait = self._fetch_words(rows.flat, "_score_ring")
+        return lambda: wait().copy()
 
     def _sample(self, logits, ctx, sample):
         """Draw the token of every wanted row on the device (ops.sample) from its request's sampler state."""

@@ -78,3 +78,20 @@ class LmHead(Part):
         logits = ctx.buf("logits", (n, self.vocab), torch.float32)
         ops.linear(h, self.weight, logits, softcap=self.softcap)
         return logits
+
+    def score(self, x: torch.Tensor, ctx, tokens: torch.Tensor, rows) -> None:
+        """What the model says about `tokens[i]` at the i-th wanted place, into `rows` (sampling/scores.py).  Without alternatives the
+        logits are never stored and there are no ranks (-1); with them they are, a piece of the rows at a time."""
+        n = ctx.n_logits
+        h = self.norm.forward(x, ctx, ctx.act_dtype, rows=ctx.logit_rows)
+        if not rows.top:
+            rows.rank.fill_(-1)
+            ops.head_logprobs(h, self.weight, tokens, rows.logprob, out_entropy=rows.entropy, softcap=self.softcap)
+            return
+        step = max(1, min(n, ops.LOGITS_PIECE_BYTES // (4 * self.vocab)))
+        for a in range(0, n, step):
+            b = min(n, a + step)
+            logits = ctx.buf("score_logits", (b - a, self.vocab), torch.float32)
+            ops.linear(h[a:b], self.weight, logits, softcap=self.softcap)
+            ops.token_logprobs(logits, tokens[a:b], rows.logprob[a:b], out_entropy=rows.entropy[a:b], out_rank=rows.rank[a:b],
+                               out_top_ids=rows.ids[a:b], out_top_logprobs=rows.top_logprobs[a:b])

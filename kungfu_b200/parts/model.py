@@ -95,4 +95,7 @@ class DecoderModel(Part):
         if ctx.n_logits == 0:
             return None
         with ops.nvtx_range("head"):
+            if ctx.score is not None:                     # a step that scores given tokens: no logits come back
+                self.head.score(x, ctx, *ctx.score)
+                return None
             return self.head.forward(x, ctx)
