@@ -321,18 +321,18 @@ head_logprobs_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
         for (int j = 0; j < COLS; ++j) g = j == at ? acc[j] : g;
         p.given[tt * TILE_ROWS + in_tile] = g;
       }
-      float m0 = acc[0], m1 = acc[1];
+      float m0 = -INFINITY, m1 = -INFINITY;
 #pragma unroll
-      for (int j = 2; j < COLS; j += 2) {
-        m0 = kf_row::max_nan(m0, acc[j]);
-        m1 = kf_row::max_nan(m1, acc[j + 1]);
+      for (int j = 0; j < COLS; j += 2) {
+        m0 = fmaxf(m0, acc[j]);
+        m1 = fmaxf(m1, acc[j + 1]);
       }
-      kf_row::move_to(st, kf_row::max_nan(st.m, kf_row::max_nan(m0, m1)));
+      kf_row::move_to(st, fmaxf(st.m, fmaxf(m0, m1)));
       kf_row::add_exponentials<COLS>(st, [&](int j) { return acc[j]; });
     }
     const float nan = __int_as_float(0x7fffffff);
     if (!ok)
-      for (int tt = 0; tt < n_tt; ++tt) mine[(size_t)tt * TILE_ROWS] = make_float4(nan, nan, nan, 0.f);
+      for (int tt = 0; tt < n_tt; ++tt) mine[(size_t)tt * TILE_ROWS] = make_float4(-INFINITY, nan, nan, 0.f);
     else if (tt_now >= 0)
       mine[(size_t)tt_now * TILE_ROWS] = make_float4(st.m, st.s, st.u, 0.f);
   }

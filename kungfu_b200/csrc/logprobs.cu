@@ -168,8 +168,9 @@ __device__ __noinline__ int prune(int n, int k, Shared& sh) {
   return kept;
 }
 
-template <typename T, bool RANK, bool TOP>
-__global__ void __launch_bounds__(NT, 2)
+// AHEAD: the next chunk's columns are on their way while one is worked on (two blocks an SM); else three blocks an SM.
+template <typename T, bool RANK, bool TOP, bool AHEAD>
+__global__ void __launch_bounds__(NT, AHEAD ? 2 : 3)
 token_logprobs_kernel(const T* __restrict__ logits, long ld, int V, const int* __restrict__ tokens, float* __restrict__ logprob,
                       float* __restrict__ entropy, int* __restrict__ rank_out, int top, int* __restrict__ top_ids,
                       float* __restrict__ top_logprobs, int slices) {
@@ -217,8 +218,8 @@ token_logprobs_kernel(const T* __restrict__ logits, long ld, int V, const int* _
   if (slice == 0 && tid < loose) {
     const int i = tid < head ? tid : n_vec * VN + tid;
     const float v = kf_load(x, i);
-    st.m = v;
-    st.s = v == -INFINITY ? 0.f : 1.f;
+    st.m = v == v ? v : -INFINITY;
+    st.s = v == -INFINITY ? 0.f : v == v ? 1.f : v;
     if (RANK) before = (v > given || (v == given && i < token)) ? 1 : 0;
     if (TOP && v > tau) sh.keys[atomicAdd(&sh.n_keys, 1)] = rank_key(v, (unsigned)i);
   }
@@ -226,13 +227,14 @@ token_logprobs_kernel(const T* __restrict__ logits, long ld, int V, const int* _
 #pragma unroll 1
   for (int c = v_begin; c < v_end; c += STEP) {
     uint4 next[NV];
-    load(c + STEP, next);                                     // (nothing is read beyond the slice)
-    float cm = Vec<T>::get(raw[0], 0);
+    if (AHEAD) load(c + STEP, next);                          // (nothing is read beyond the slice)
+    else if (c > v_begin) load(c, raw);
+    float cm = -INFINITY;
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
-      for (int e = 0; e < VN; ++e) cm = max_nan(cm, Vec<T>::get(raw[j], e));
-    move_to(st, max_nan(st.m, cm));
+      for (int e = 0; e < VN; ++e) cm = fmaxf(cm, Vec<T>::get(raw[j], e));
+    move_to(st, fmaxf(st.m, cm));
     add_exponentials<PER_THREAD>(st, [&](int i) { return Vec<T>::get(raw[i / VN], i % VN); });
     if (RANK) {
       // Columns before the token count when they equal it, columns behind it do not: they must exceed the next lower number, or the
@@ -262,7 +264,7 @@ token_logprobs_kernel(const T* __restrict__ logits, long ld, int V, const int* _
       // Every column above `limit` becomes a key; returns how long the warp saw the list get.  A key that finds the list full is not
       // written, and the length tells.
       auto push = [&](float limit) {
-        if (__ballot_sync(0xffffffffu, !(cm <= limit)) == 0u) return 0;
+        if (__ballot_sync(0xffffffffu, cm > limit) == 0u) return 0;
         unsigned hits = 0u;
 #pragma unroll
         for (int j = 0; j < NV; ++j)
@@ -296,7 +298,7 @@ token_logprobs_kernel(const T* __restrict__ logits, long ld, int V, const int* _
       float limit = tau;
       bool bounded = false;
       if (c == v_begin) {
-        limit = nextafterf(warp_bound(cm == cm ? cm : -INFINITY, top, sh), -INFINITY);
+        limit = nextafterf(warp_bound(cm, top, sh), -INFINITY);
         bounded = true;
       }
       for (;;) {
@@ -313,7 +315,7 @@ token_logprobs_kernel(const T* __restrict__ logits, long ld, int V, const int* _
         n = compact(KEY_CAP, -INFINITY, id0, id1, sh);
         if (n >= top) settle(prune(n, top, sh));
         if (!bounded) {
-          limit = fmaxf(tau, nextafterf(warp_bound(cm == cm ? cm : -INFINITY, top, sh), -INFINITY));
+          limit = fmaxf(tau, nextafterf(warp_bound(cm, top, sh), -INFINITY));
           bounded = true;
           continue;
         }
@@ -336,8 +338,10 @@ token_logprobs_kernel(const T* __restrict__ logits, long ld, int V, const int* _
         break;
       }
     }
+    if (AHEAD) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j) raw[j] = next[j];
+      for (int j = 0; j < NV; ++j) raw[j] = next[j];
+    }
   }
 
   // the block's numbers, then the cluster's
@@ -431,7 +435,7 @@ token_logprobs_kernel(const T* __restrict__ logits, long ld, int V, const int* _
   }
 }
 
-template <typename T, bool RANK, bool TOP>
+template <typename T, bool RANK, bool TOP, bool AHEAD>
 int launch(const void* logits, long ld, int R, int V, const int* tokens, float* logprob, float* entropy, int* rank, int top,
            int* top_ids, float* top_logprobs, int slices, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
@@ -444,7 +448,7 @@ int launch(const void* logits, long ld, int R, int V, const int* tokens, float* 
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev < 0 || dev >= 64 || !allowed[dev]) {
-      if (cudaFuncSetAttribute(token_logprobs_kernel<T, RANK, TOP>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
+      if (cudaFuncSetAttribute(token_logprobs_kernel<T, RANK, TOP, AHEAD>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
         kf_record_cuda_error(cudaGetLastError());
         return KF_ERR_SETUP;
       }
@@ -459,19 +463,18 @@ int launch(const void* logits, long ld, int R, int V, const int* tokens, float* 
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = kf_pdl_enabled() ? 2 : 1;
-  cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, RANK, TOP>, (const T*)logits, ld, V, tokens, logprob, entropy, rank, top, top_ids,
+  cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, RANK, TOP, AHEAD>, (const T*)logits, ld, V, tokens, logprob, entropy, rank, top, top_ids,
                      top_logprobs, slices);
   KF_CHECK_LAUNCH();
   return KF_OK;
 }
 
-template <typename T>
+template <typename T, bool AHEAD>
 int launch_type(const void* logits, long ld, int R, int V, const int* tokens, float* logprob, float* entropy, int* rank, int top,
                 int* top_ids, float* top_logprobs, int slices, cudaStream_t stream) {
-  if (rank && top) return launch<T, true, true>(logits, ld, R, V, tokens, logprob, entropy, rank, top, top_ids, top_logprobs, slices, stream);
-  if (rank) return launch<T, true, false>(logits, ld, R, V, tokens, logprob, entropy, rank, top, top_ids, top_logprobs, slices, stream);
-  if (top) return launch<T, false, true>(logits, ld, R, V, tokens, logprob, entropy, rank, top, top_ids, top_logprobs, slices, stream);
-  return launch<T, false, false>(logits, ld, R, V, tokens, logprob, entropy, rank, top, top_ids, top_logprobs, slices, stream);
+  const auto f = rank ? (top ? launch<T, true, true, AHEAD> : launch<T, true, false, AHEAD>)
+                      : (top ? launch<T, false, true, AHEAD> : launch<T, false, false, AHEAD>);
+  return f(logits, ld, R, V, tokens, logprob, entropy, rank, top, top_ids, top_logprobs, slices, stream);
 }
 
 }  // namespace
@@ -497,9 +500,12 @@ KF_API int kf_token_logprobs(const void* logits, int dt, long ld, int R, int V, 
 #ifdef KF_TUNING
   if (g_slices > 0) slices = g_slices;
 #endif
-  if (dt == KF_F32)
-    return launch_type<float>(logits, ld, R, V, tokens, logprob, entropy, rank, top, top_ids, top_logprobs, slices, stream);
-  if (dt == KF_BF16)
-    return launch_type<__nv_bfloat16>(logits, ld, R, V, tokens, logprob, entropy, rank, top, top_ids, top_logprobs, slices, stream);
-  return KF_ERR_DTYPE;
+  // Rows of a few chunks that need more than two blocks an SM: a block's start and end are most of its time, and a third block hides more of
+  // them than loads ahead do.  2,048 x 32,000 with 20 alternatives 100 us ahead, 92 not, without alternatives 57 and 54; 301 x 32,003 with
+  // 64 alternatives 38 and 35; 512 x 256,000 89 and 115.
+  const bool ahead = kf_ceil_div(chunks, slices) > 4 || (long)R * slices <= 2l * kf_sm_count();
+  if (dt != KF_F32 && dt != KF_BF16) return KF_ERR_DTYPE;
+  const auto f = dt == KF_F32 ? (ahead ? launch_type<float, true> : launch_type<float, false>)
+                              : (ahead ? launch_type<__nv_bfloat16, true> : launch_type<__nv_bfloat16, false>);
+  return f(logits, ld, R, V, tokens, logprob, entropy, rank, top, top_ids, top_logprobs, slices, stream);
 }

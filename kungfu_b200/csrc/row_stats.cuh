@@ -7,6 +7,7 @@ namespace kf_row {
 typedef unsigned long long u64;
 constexpr float LOG2E = 1.4426950408889634f;
 
+// max(a, b), NaN if either is
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -45,7 +46,8 @@ __device__ __forceinline__ u64 fma2(u64 a, u64 b, u64 c) {
   return r;
 }
 
-// Running maximum, sum of exponentials and sum of d exp(d), and how a second set joins the first.
+// Running maximum (of what is a number), sum of exponentials and sum of d exp(d), and how a second set joins the first.  A NaN
+// among the logits is a NaN in s.
 struct Stats { float m, s, u; };
 __device__ __forceinline__ void move_to(Stats& a, float m) {
   if (m != a.m) {
@@ -56,7 +58,7 @@ __device__ __forceinline__ void move_to(Stats& a, float m) {
   }
 }
 __device__ __forceinline__ void join(Stats& a, Stats b) {
-  const float m = max_nan(a.m, b.m);
+  const float m = fmaxf(a.m, b.m);
   move_to(a, m);
   move_to(b, m);
   a.s += b.s;
@@ -74,7 +76,7 @@ __device__ __forceinline__ void add_exponentials(Stats& a, F get) {
 #pragma unroll
   for (int i = 0; i < N; i += 2) {
     float2 d = unpack2(add2(pack2(get(i), get(i + 1)), minus));
-    const u64 low = pack2(fmaxf(d.x, -200.f), fmaxf(d.y, -200.f));
+    const u64 low = pack2(max_nan(d.x, -200.f), max_nan(d.y, -200.f));
     d = unpack2(mul2(low, scale));
     const u64 w = pack2(exp2_fast(d.x), exp2_fast(d.y));
     s2 = add2(s2, w);
@@ -85,14 +87,15 @@ __device__ __forceinline__ void add_exponentials(Stats& a, F get) {
   a.u += u.x + u.y;
 }
 
-// The results for a token whose logit is `given` (NaN for one that is no column).
+// The results for a token whose logit is `given` (NaN for one that is no column).  NaN and +inf among the logits give NaN.
+__device__ __forceinline__ bool is_no_distribution(const Stats& a) { return a.s != a.s || a.m == INFINITY; }
 __device__ __forceinline__ float row_logprob(const Stats& a, float given) {
-  const float m = a.m == INFINITY ? __int_as_float(0x7fffffff) : a.m;
-  if (m == -INFINITY) return given == given ? -INFINITY : given;
-  return (given - m) - logf(a.s);
+  if (is_no_distribution(a)) return __int_as_float(0x7fffffff);
+  if (a.m == -INFINITY) return given == given ? -INFINITY : given;
+  return (given - a.m) - logf(a.s);
 }
 __device__ __forceinline__ float row_entropy(const Stats& a) {
-  if (a.m == INFINITY) return __int_as_float(0x7fffffff);
+  if (is_no_distribution(a)) return __int_as_float(0x7fffffff);
   return a.m == -INFINITY ? 0.f : logf(a.s) - a.u / a.s;
 }
 
