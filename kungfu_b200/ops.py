@@ -10,6 +10,7 @@ from __future__ import annotations
 import ctypes
 import os
 import threading
+from array import array
 
 import torch
 
@@ -1480,6 +1481,7 @@ def token_logprobs(logits, tokens, out_logprob, *, out_entropy=None, out_rank=No
                                        _address(out_top_logprobs), stream), what)
 
 
+HEAD_ROWS = 16384               # rows of one launch of the fused kernel: a workspace of 40 MB at most
 LOGITS_PIECE_BYTES = 256 << 20  # logits held at a time where `head_logprobs` computes them first
 
 
@@ -1508,15 +1510,23 @@ def head_logprobs(x, weight, tokens, out_logprob, *, out_entropy=None, softcap: 
     if use_tensor_cores and x.dtype == torch.bfloat16 and weight.dtype == torch.bfloat16:
         lib = library()
         if lib.kf_head_logprobs_supported(x.data_ptr(), weight.data_ptr(), K):
-            # its own workspace for every call: calls on several streams, and graphs replayed at a time, do not share sums
-            work = torch.empty(lib.kf_head_logprobs_workspace(R, V), dtype=torch.float32, device=x.device)
-            _check(lib.kf_head_logprobs(x.data_ptr(), weight.data_ptr(), tokens.data_ptr(), R, V, K, softcap, out_logprob.data_ptr(),
-                                        _address(out_entropy), work.data_ptr(), _dev_scratch(x.device)["error"].data_ptr(), stream), what)
-            add_launches(1)
+            error = _dev_scratch(x.device)["error"].data_ptr()
+            for a in range(0, R, HEAD_ROWS):
+                n, size = min(HEAD_ROWS, R - a), x.element_size()
+                # its own workspace for every call: calls on several streams, and graphs replayed at a time, do not share sums
+                work = torch.empty(lib.kf_head_logprobs_workspace(n, V), dtype=torch.float32, device=x.device)
+                _check(lib.kf_head_logprobs(x.data_ptr() + a * K * size, weight.data_ptr(), tokens.data_ptr() + 4 * a, n, V, K, softcap,
+                                            out_logprob.data_ptr() + 4 * a, None if out_entropy is None else out_entropy.data_ptr() + 4 * a,
+                                            work.data_ptr(), error, stream), what)
+                add_launches(1)
             return
         note_fallback(f"{what}: rows of {K} bfloat16 elements are no multiple of 16 bytes (or a base is unaligned)")
     step = max(1, min(R, LOGITS_PIECE_BYTES // (4 * V)))
     logits = torch.empty((step, V), dtype=torch.float32, device=x.device)
+    if step == R:
+        linear(x, weight, logits, softcap=softcap)
+        token_logprobs(logits, tokens, out_logprob, out_entropy=out_entropy)
+        return
     for a in range(0, R, step):
         b = min(R, a + step)
         linear(x[a:b], weight, logits[:b - a], softcap=softcap)
@@ -1554,13 +1564,11 @@ def copy_pages(stores, src, dst) -> None:
         return
     stream = _current(what, device)
     lib = library()
-    for a in range(0, len(bases), 64):
-        m = min(64, len(bases) - a)
-        at, of = (ctypes.c_int64 * m)(*bases[a:a + m]), (ctypes.c_int64 * m)(*sizes[a:a + m])
+    at, of, src, dst = array("q", bases), array("q", sizes), array("i", src), array("i", dst)
+    at0, of0, src0, dst0 = (x.buffer_info()[0] for x in (at, of, src, dst))
+    for a in range(0, len(bases), 64):                         # what one launch takes: 64 stores and 256 pairs
         for i in range(0, n, 256):
-            k = min(256, n - i)
-            ids = ctypes.c_int * k
-            _check(lib.kf_copy_pages(at, of, m, ids(*src[i:i + k]), ids(*dst[i:i + k]), k, stream), what)
+            _check(lib.kf_copy_pages(at0 + 8 * a, of0 + 8 * a, min(64, len(bases) - a), src0 + 4 * i, dst0 + 4 * i, min(256, n - i), stream), what)
 
 
 def device_arch() -> int:

@@ -91,6 +91,18 @@ def test_whole_vocabulary():
     check(*make(70, 2304, 256000, torch.bfloat16), 30.0)
 
 
+def test_more_rows_than_one_launch_takes(monkeypatch):
+    from kungfu_b200 import ops
+    x, w, t = make(700, 64, 3000, torch.bfloat16)
+    for rows in (256, 100):                                   # (which worker sums which tile depends on the rows of a launch: not the same bits)
+        monkeypatch.setattr(ops, "HEAD_ROWS", rows)
+        check(x, w, t, 30.0)
+    xf, wf = x.float(), w.float()
+    whole = run(xf, wf, t, 30.0)
+    monkeypatch.setattr(ops, "LOGITS_PIECE_BYTES", 100 * 4 * 3000)
+    assert all(torch.equal(a, b) for a, b in zip(run(xf, wf, t, 30.0), whole))
+
+
 def test_padding_rows_and_strange_tokens():
     x, w, t = make(150, 128, 3001, torch.bfloat16)
     whole, ent = run(x, w, t, 0.0)
