@@ -120,7 +120,7 @@ head_logprobs_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < p.stages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-    for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], (PAIR ? 2 : 1) * 32 * EPI_WARPS); }
+    for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], (PAIR ? 2 : 1) * EPI_WARPS); }
     *s_abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -259,12 +259,15 @@ head_logprobs_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
           break;
         }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        auto release = [&]() {
+        auto release = [&]() {                                    // one arrival a warp: 16 of a pair's, not 512, meet at the leader's barrier
           asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-          if (PAIR)
-            asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(in_leader(smem_u32(&acc_empty[buf]))) : "memory");
-          else
-            mbar_arrive(&acc_empty[buf]);
+          __syncwarp();
+          if (lane == 0) {
+            if (PAIR)
+              asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(in_leader(smem_u32(&acc_empty[buf]))) : "memory");
+            else
+              mbar_arrive(&acc_empty[buf]);
+          }
         };
         if (idle) {
           release();
