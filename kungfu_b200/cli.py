@@ -142,6 +142,8 @@ PARAMS = [
     ("min_p", "float", "0", "--min-p", "zero disables"),
     ("repeat_penalty", "float", "1", "--repeat-penalty", "one disables"),
     ("max_tokens", "int", "64", "--max-tokens", "tokens generated per request"),
+    ("beams", "int", "1", "--beams", "open answers of a beam search, one for sampling"),
+    ("logprobs", "int", "", "--logprobs", "alternatives reported with every generated token, none without it"),
 ]
 
 

@@ -15,6 +15,8 @@
 // column must exceed to join them.  The first chunk is cut by a bound that at least k of its columns reach (`warp_bound`) and
 // leaves the exact k-th value as tau.  From then on a column costs one comparison (of the thread's maximum), and a random row
 // brings k * 8,192 / (columns seen) keys a chunk; a list grown long is pruned to its k best, which raises tau.
+// What bounds it: memory for long rows without alternatives (512 x 256,000 in 89 us, 5.9 TB/s); with them the first chunk's bound and
+// ranking and the row's last ranking, which its loads do not cover (512 rows with 20 alternatives 131 us, 64 rows 32, one row 16).
 #include "row_stats.cuh"
 
 namespace {
@@ -171,15 +173,16 @@ __device__ __noinline__ int prune(int n, int k, Shared& sh) {
 // AHEAD: the next chunk's columns are on their way while one is worked on (two blocks an SM); else three blocks an SM.
 template <typename T, bool RANK, bool TOP, bool AHEAD>
 __global__ void __launch_bounds__(NT, AHEAD ? 2 : 3)
-token_logprobs_kernel(const T* __restrict__ logits, long ld, int V, const int* __restrict__ tokens, float* __restrict__ logprob,
-                      float* __restrict__ entropy, int* __restrict__ rank_out, int top, int* __restrict__ top_ids,
-                      float* __restrict__ top_logprobs, int slices) {
+token_logprobs_kernel(const T* logits, long ld, int V, const int* tokens, float* __restrict__ logprob, float* __restrict__ entropy,
+                      int* __restrict__ rank_out, int top, int* __restrict__ top_ids, float* __restrict__ top_logprobs, int slices) {
   constexpr int VN = Vec<T>::N, NV = PER_THREAD / VN, STEP = NT * NV;
   extern __shared__ __align__(16) unsigned char cluster_raw[];       // a ClusterShared where a cluster shares a row
   __shared__ Shared sh;
   kf_pdl_trigger();
   if (slices > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");      // waited for before a peer's memory is touched
   kf_pdl_wait();
+  logits = kf_produced(logits);                               // no load may stand above the wait
+  tokens = kf_produced(tokens);
   const int row = (int)(blockIdx.x / (unsigned)slices), slice = (int)(blockIdx.x % (unsigned)slices);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int token = tokens ? tokens[row] : 0;

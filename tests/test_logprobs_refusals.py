@@ -56,3 +56,12 @@ def test_there_is_no_cpu_path():
                  lambda: ops.copy_pages([_t(4, 2)], [0], [1])):
         with pytest.raises(KernelError, match="CUDA"):
             call()
+
+
+def test_tensors_of_another_device_than_the_current_one_are_refused(monkeypatch):
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 1)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    with pytest.raises(KernelError, match="current device is cuda:1"):
+        ops._current("token_logprobs", 0)
+    with pytest.raises(KernelError, match="another device"):
+        ops._checked("token_logprobs", 0, (("tokens", _t(4, dtype=I32), (4,), I32),))
