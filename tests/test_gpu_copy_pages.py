@@ -15,7 +15,8 @@ def check(stores, src, dst):
     ops.copy_pages(stores, src, dst)
     torch.cuda.synchronize()
     for a, b in zip(stores, want):
-        assert torch.equal(a.view(torch.uint8) if a.dtype == torch.bfloat16 else a, b.view(torch.uint8) if b.dtype == torch.bfloat16 else b)
+        bits = {torch.bfloat16: torch.int16, torch.float32: torch.int32}.get(a.dtype, a.dtype)
+        assert torch.equal(a.view(bits), b.view(bits))
 
 
 def _store(g, n, shape, dtype):
@@ -54,6 +55,20 @@ def test_a_base_that_is_not_aligned():
         before = flat.clone()
         check([flat[off:off + 10 * n].view(10, n)], [0, 9], [4, 5])
         assert torch.equal(flat[:off], before[:off]) and torch.equal(flat[off + 10 * n:], before[off + 10 * n:])
+
+
+def test_every_phase_of_sixteen_bytes():
+    """Sources and copies at every pair of phases, of pages with and without a whole vector between their ends; the bytes around them stay."""
+    g = torch.Generator().manual_seed(9)
+    flat = torch.randint(0, 255, (16 + 33 * 40000,), generator=g).to(torch.uint8).to(DEV)
+    for n in (1, 2, 15, 16, 17, 30, 31, 33, 47, 48, 49, 63, 65, 95, 16384 + 16 + 1, 16384 + 47):
+        for off in (0, 1, 2, 4, 7, 8, 12, 15):
+            before = flat.clone()
+            check([flat[off:off + 33 * n].view(33, n)], list(range(16)), list(range(16, 32)))
+            assert torch.equal(flat[:off], before[:off]) and torch.equal(flat[off + 33 * n:], before[off + 33 * n:])
+    for dtype, size in ((torch.bfloat16, 2), (torch.float32, 4)):
+        for n in (1, 3, 9, 13, 8197, 8191):
+            check([_store(g, 33, (n,), dtype), flat[:33 * n * size + size].view(dtype)[1:1 + 33 * n].view(33, n)], list(range(16)), list(range(16, 32)))
 
 
 def test_nothing_to_copy():
