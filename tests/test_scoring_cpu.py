@@ -301,6 +301,60 @@ def test_a_forked_request_goes_on_by_itself(model, cpu_ops, pipeline):
         eng.fork(a)                                           # finished
 
 
+def test_forks_that_outgrow_the_pool_are_preempted_and_recomputed(model, cpu_ops):
+    folder, cfg, tensors = model
+    prompt = helpers.random_tokens(5, 512, 8)
+    want = plain_gemma2.greedy(cfg, tensors, prompt, 12)
+    eng = _engine(folder, cfg, pool_tokens=36, batch=16)      # nine pages: four requests of 17 tokens want up to twenty
+    a = eng.add_request(prompt, Sampling(temperature=0.0), max_tokens=12, ignore_eos=True, logprobs=0)
+    while len(eng.requests[a].output) < 2:
+        eng.step()
+    ids = [a, eng.fork(a), eng.fork(a), eng.fork(a)]
+    while not eng.idle:
+        eng.step()
+        eng.runner.cache.check()
+    assert eng.scheduler.n_preemptions > 0
+    for i in ids:
+        assert eng.requests[i].output == want and len(eng.requests[i].scores) == 12
+    assert eng.runner.cache.free_pages() == [9, 9]
+
+
+def test_a_cancelled_parent_leaves_its_forks_alone(model, cpu_ops):
+    folder, cfg, tensors = model
+    prompt = helpers.random_tokens(10, 512, 9)
+    want = plain_gemma2.greedy(cfg, tensors, prompt, 8)
+    eng = _engine(folder, cfg)
+    a = eng.add_request(prompt, Sampling(temperature=0.0), max_tokens=8, ignore_eos=True)
+    while len(eng.requests[a].output) < 3:
+        eng.step()
+    b = eng.fork(a)
+    events = eng.cancel(a)
+    assert (a, None, "cancelled") in events
+    other = eng.add_request(helpers.random_tokens(30, 512, 1), Sampling(temperature=0.0), max_tokens=4, ignore_eos=True)    # takes what came back
+    while not eng.idle:
+        eng.step()
+    assert eng.requests[b].output == want and len(eng.requests[other].output) == 4
+    eng.runner.cache.check()
+
+
+@pytest.mark.parametrize("pipeline", [True, False])
+def test_scoring_and_searching_beside_running_requests(model, cpu_ops, pipeline):
+    folder, cfg, tensors = model
+    prompt, text = helpers.random_tokens(9, 512, 2), helpers.random_tokens(21, 512, 5)
+    want = plain_gemma2.greedy(cfg, tensors, prompt, 10)
+    eng = _engine(folder, cfg, pipeline=pipeline, parallel=6)
+    a = eng.add_request(prompt, Sampling(temperature=0.0), max_tokens=10, ignore_eos=True)
+    events = eng.step() + eng.step() + eng.step()
+    scores = eng.score([text])[0]
+    assert all(abs(s.logprob - w[0]) < TOL for s, w in zip(scores, sc.plain_scores(cfg, tensors, text)))
+    events += eng.step() + eng.step()
+    found = eng.beam_search(text, beams=4, max_tokens=4, ignore_eos=True)
+    assert [b.tokens for b in found] == [t for t, _, _ in sc.plain_beams(cfg, tensors, text, 4, 4)]
+    while not eng.idle:
+        events += eng.step()
+    assert eng.requests[a].output == want and [t for i, t, _ in events if i == a] == want
+
+
 def test_forks_without_a_slot_are_refused(model, cpu_ops):
     folder, cfg, _ = model
     eng = _engine(folder, cfg, parallel=2)
