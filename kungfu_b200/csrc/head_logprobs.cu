@@ -77,10 +77,11 @@ __device__ __forceinline__ float min_nan(float a, float b) {
   return r;
 }
 // 1 / d for d in [1, 2^41], two at a time on the FMA units (the hardware's reciprocal shares its unit with the exponential, which bounds
-// the epilogue): a first guess from the bits, within 6 %, and three Newton steps r (2 - d r), each of which squares the error.
+// the epilogue): a first guess from the exponent's and fraction's bits (of all constants to subtract them from, the one whose
+// largest error is least, 5.1 %), and three Newton-Raphson steps r (2 - d r), each of which squares the error.
 __device__ __forceinline__ u64 reciprocal2(u64 d) {
   const float2 f = kf_row::unpack2(d);
-  u64 r = kf_row::pack2(__int_as_float(0x7ef311c3 - __float_as_int(f.x)), __int_as_float(0x7ef311c3 - __float_as_int(f.y)));
+  u64 r = kf_row::pack2(__int_as_float(0x7ef31200 - __float_as_int(f.x)), __int_as_float(0x7ef31200 - __float_as_int(f.y)));
   const u64 minus = kf_row::pack2(-f.x, -f.y), two = kf_row::pack2(2.f, 2.f);
 #pragma unroll
   for (int i = 0; i < 3; ++i) r = kf_row::mul2(r, kf_row::fma2(minus, r, two));
