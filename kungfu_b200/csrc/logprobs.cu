@@ -29,6 +29,7 @@ constexpr int PER_THREAD = 32;                               // columns of a chu
 constexpr int CHUNK = NT * PER_THREAD;
 constexpr int MAX_SLICES = 16;
 constexpr int KEY_CAP = NT * 8 + TOP_MAX;                    // keys held at most: a vector of every thread beside the k best
+constexpr int TAIL_MAX = 7;                                  // columns behind a row's last vector; the list has room for them besides
 constexpr int FEW_KEYS = 256;                                // up to here keys are ranked by counting the larger ones at once
 
 __device__ __forceinline__ unsigned orderable(float v) {     // larger float <=> larger unsigned; -0 as +0; NaN below everything
@@ -85,7 +86,7 @@ struct Shared {
   float bound[WARPS];
   int n_keys;
   u64 sorted[TOP_MAX];
-  u64 keys[KEY_CAP];
+  u64 keys[KEY_CAP + TAIL_MAX];
 };
 struct ClusterShared {                                        // what the row's blocks leave with the first one
   Stats stats[MAX_SLICES];
@@ -117,7 +118,7 @@ __device__ __noinline__ float warp_bound(float mine, int k, Shared& sh) {
 // Of the keys in the list [0, n), those of at least `bound` and whose ids are not in [id0, id1), moved to its front; returns how
 // many.  All threads call it.
 __device__ __noinline__ int compact(int n, float bound, unsigned id0, unsigned id1, Shared& sh) {
-  constexpr int MINE = (KEY_CAP + NT - 1) / NT;
+  constexpr int MINE = (KEY_CAP + TAIL_MAX + NT - 1) / NT;
   const int tid = threadIdx.x;
   u64 mine[MINE];
 #pragma unroll
@@ -190,7 +191,7 @@ token_logprobs_kernel(const T* logits, long ld, int V, const int* tokens, float*
   const T* x = logits + (size_t)row * ld;
   const bool inside = token < V;
 
-  // The row: `head` elements up to a 16-byte boundary, `n_vec` vectors, the rest.  Loose elements go to the first slice.
+  // The row: `head` elements up to a 16-byte boundary, `n_vec` vectors, the tail.  Loose elements go to the first slice.
   const int head = min(V, (int)((16 - ((uintptr_t)x & 15)) % 16 / sizeof(T)));
   const int n_vec = (V - head) / VN, loose = V - n_vec * VN;
   const T* body = x + head;
@@ -224,7 +225,7 @@ token_logprobs_kernel(const T* logits, long ld, int V, const int* tokens, float*
     st.m = v == v ? v : -INFINITY;
     st.s = v == -INFINITY ? 0.f : v == v ? 1.f : v;
     if (RANK) before = (v > given || (v == given && i < token)) ? 1 : 0;
-    if (TOP && v > tau) sh.keys[atomicAdd(&sh.n_keys, 1)] = rank_key(v, (unsigned)i);
+    if (TOP && tid < head && v > tau) sh.keys[atomicAdd(&sh.n_keys, 1)] = rank_key(v, (unsigned)i);
   }
 
 #pragma unroll 1
@@ -347,6 +348,13 @@ token_logprobs_kernel(const T* logits, long ld, int V, const int* tokens, float*
     }
   }
 
+  // The tail's ids are the highest: its keys come last, so that a column that equals tau has a higher id than the key that set it.
+  if (TOP && slice == 0 && tid >= head && tid < loose) {
+    const int i = n_vec * VN + tid;
+    const float v = kf_load(x, i);
+    if (v > tau) sh.keys[atomicAdd(&sh.n_keys, 1)] = rank_key(v, (unsigned)i);
+  }
+
   // the block's numbers, then the cluster's
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
@@ -361,7 +369,7 @@ token_logprobs_kernel(const T* logits, long ld, int V, const int* tokens, float*
   __syncthreads();
   int n = 0;
   if (TOP) {
-    n = sh.n_keys;                                            // within the list's room after every chunk
+    n = sh.n_keys;                                            // within KEY_CAP after every chunk, and the tail
     __syncthreads();
     n = prune(n, top, sh);
   }
