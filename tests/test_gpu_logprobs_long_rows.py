@@ -1,4 +1,5 @@
-"""Rows of several chunks a block whose length or start is no multiple of 16 bytes: ties across their ends, lists of keys that grow too long."""
+"""Rows of several chunks a block whose length or start is no multiple of 16 bytes: ties across their ends, lists of keys that grow too long,
+masks of the lowest number."""
 import pytest
 import torch
 
@@ -84,3 +85,18 @@ def test_shapes_in_rows_of_several_chunks(R, V, top, skip, dtype):
     rows = torch.stack([kinds[r % len(kinds)] for r in range(R)])
     tokens = torch.tensor([(0, V // 2, V - 1, 8192 + 3)[r // len(kinds) % 4] for r in range(R)], dtype=torch.int32)
     check(_apart(rows, skip, dtype), tokens.to(DEV), top)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("low", ["lowest", -3e38, -1e38])
+@pytest.mark.parametrize("R,V", [(7, 5001), (7, 40000), (1, 256003), (160, 32003), (320, 24581)])
+def test_masks_of_the_lowest_number_over_ranges(R, V, low, dtype):
+    """A mask of finite numbers whose sum over a thread's columns is none: its range first, last, all but one column, by chunks and by stripes."""
+    low = torch.finfo(dtype).min if low == "lowest" else low
+    g = torch.Generator().manual_seed(V)
+    r, i = 3.0 * torch.randn(V, generator=g), torch.arange(V)
+    masks = [i < V // 2, i >= V // 2, i != V // 2, i != V - 1, i < 8192, i // 8192 % 2 == 0, i // 32 % 2 == 0]
+    rows = torch.stack([torch.where(masks[n % len(masks)], torch.tensor(low), r) for n in range(max(R, len(masks)))])
+    for a in range(0, rows.shape[0], R):                      # (one row at a time where a row is shared by a cluster)
+        x = _apart(rows[a:a + R], 0, dtype)
+        check(x, torch.full((x.shape[0],), V // 3, dtype=torch.int32, device=DEV), 3)
