@@ -5,7 +5,8 @@
 //   with d_j = x_j - max, s = sum_j exp(d_j);   rank of t = how many columns come before it (larger, or equal with a lower id).
 //
 // Both terms of H are >= 0, so nothing cancels.  A row whose every column is -inf has no distribution: its log probabilities
-// are -inf and its entropy 0.  A row that holds NaN or +inf gives NaN.  NaN ranks behind -inf among the alternatives.
+// are -inf and its entropy 0.  A row that holds NaN or +inf gives NaN; a token whose own logit is NaN has no rank (-1).  NaN comes
+// behind -inf among the alternatives.
 //
 // Shape.  A row is read once.  A block walks its slice of the row in chunks of 8,192 columns, 32 in the registers of each
 // thread (the next chunk's on their way), and keeps per thread the running maximum m, s and u = sum d exp(d) (a new maximum moves
@@ -437,7 +438,7 @@ token_logprobs_kernel(const T* logits, long ld, int V, const int* tokens, float*
   if (tid == 0) {
     if (logprob) logprob[row] = row_logprob(st, inside ? given : __int_as_float(0x7fffffff));
     if (entropy) entropy[row] = row_entropy(st);
-    if (RANK) rank_out[row] = inside ? before : -1;
+    if (RANK) rank_out[row] = inside && given == given ? before : -1;
   }
   if (TOP && tid < top) {
     const u64 key = sh.sorted[tid];
@@ -496,7 +497,7 @@ KF_API void kf_token_logprobs_slices(int n) { g_slices = n; }
 #endif
 
 // logits [R, V] of element type dt (KF_F32, KF_BF16), rows ld elements apart; tokens [R] (null: only entropy and alternatives;
-// a negative one: the row's outputs stay as they are; one >= V: NaN and rank -1); every output may be null; top <= 64, <= V.
+// a negative one: the row's outputs stay as they are; one >= V, or one whose logit is NaN: NaN and rank -1); every output may be null; top <= 64, <= V.
 KF_API int kf_token_logprobs(const void* logits, int dt, long ld, int R, int V, const int* tokens, float* logprob, float* entropy,
                              int* rank, int top, int* top_ids, float* top_logprobs, cudaStream_t stream) {
   if (R <= 0) return KF_OK;

@@ -1450,7 +1450,7 @@ def token_logprobs(logits, tokens, out_logprob, *, out_entropy=None, out_rank=No
 
     A negative token leaves its row's outputs as they are (a row of padding).  A token of V or more gives NaN and rank -1.  Columns
     of -inf are masked: they have no probability; a row of nothing else gives -inf and entropy 0.  A row with NaN or +inf gives NaN,
-    and NaN comes last among the alternatives."""
+    a token whose own logit is NaN the rank -1, and NaN comes last among the alternatives."""
     what = "token_logprobs"
     if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16):
         raise KernelError(f"{what}: logits are {tuple(logits.shape)} {logits.dtype}, not rows of float32 or bfloat16")

@@ -1,9 +1,11 @@
 """Rows of several chunks a block whose length or start is no multiple of 16 bytes: ties across their ends, lists of keys that grow too long,
-masks of the lowest number."""
+masks of the lowest number, and tokens whose logit is none."""
+import math
+
 import pytest
 import torch
 
-from test_gpu_token_logprobs import DEV, _shapes, check
+from test_gpu_token_logprobs import DEV, _shapes, check, run
 
 pytestmark = pytest.mark.gpu
 
@@ -100,3 +102,16 @@ def test_masks_of_the_lowest_number_over_ranges(R, V, low, dtype):
     for a in range(0, rows.shape[0], R):                      # (one row at a time where a row is shared by a cluster)
         x = _apart(rows[a:a + R], 0, dtype)
         check(x, torch.full((x.shape[0],), V // 3, dtype=torch.int32, device=DEV), 3)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("R,V", [(6, 37), (6, 5001), (6, 120000), (160, 32003)])
+def test_a_token_whose_logit_is_no_number_has_no_rank(R, V, dtype):
+    g = torch.Generator().manual_seed(V)
+    x = torch.randn(R, V, generator=g).to(dtype)
+    tokens = torch.randint(0, V, (R,), generator=g)
+    x[torch.arange(0, R, 2), tokens[::2]] = float("nan")
+    lp, ent, rank, _, _ = run(x.to(DEV), tokens.to(torch.int32).to(DEV), 2)
+    assert rank[::2].tolist() == [-1] * len(tokens[::2])
+    assert bool(torch.isnan(lp[::2]).all()) and bool(torch.isnan(ent[::2]).all())
+    assert int(rank[1::2].min()) >= 0 and math.isfinite(float(lp[1::2].sum()))
