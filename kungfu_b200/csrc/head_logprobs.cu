@@ -8,9 +8,10 @@
 // (vocabulary tile, token tile), token tiles fastest, so that the blocks side by side read the same weights, which come from
 // memory once, and all of x, which stays in L2.  Warp 0 issues the TMA loads, warp 1 the MMAs, warps 2 to 9 drain.
 //
-// The tensor cores' 32-bit accumulators round towards zero at every step of 16 products, always shrinking the sum: over K = 2304 the
-// log probabilities were off by 2e-6 of their size.  So a tile's K is cut into runs of at most 512: two accumulators in tensor
-// memory take turns, and a run's sum is drained into 32-bit registers, rounded to nearest there, while the next run is multiplied.
+// The tensor cores' 32-bit accumulators round towards zero at every step of 16 products, always shrinking the sum: with all of K = 2304 in one
+// sum the log probabilities are off by 1.0e-6 of their size (2-norm), by 3e-6 where all products are positive.  So a tile's K is cut into runs
+// (RUN): two accumulators in tensor memory take turns, and a run's sum is drained into 32-bit registers, rounded to nearest there, while the
+// next run is multiplied.
 //
 // Every block keeps one set of statistics per token and column half, in registers while it stays on a token tile and in a
 // workspace between; a second kernel joins them.  The order of all sums is fixed by the sizes, so results repeat bit by bit.
@@ -25,7 +26,12 @@ using kf_row::Stats;
 using kf_row::u64;
 
 constexpr int BN = 256;                                         // vocabulary rows of a tile
-constexpr int RUN = 12, RUN_ALONE = 8;                          // most stages (of 64) of a run of K; of a K that is not cut
+// Most blocks of 64 of a run of K, and of a K that is not cut.  Shorter runs are more exact and more to drain.  K = 2304 over 32,000 columns, cap
+// 30: runs of 512 are off by 2.3e-7 and runs of 768 by 3.3e-7 (2-norm of the log probabilities; torch's 32-bit product and softmax by 3.4e-7 to
+// 5.1e-7).  Single blocks, which memory bounds, take 512 for nothing (40 rows over 256,000 columns 208 us either way); for pairs 768 is the
+// choice, since draining 512 at a time delays the tensor cores (2,048 rows 1,524 to 1,550 us against 1,657, 512 rows 412 to 426 against 445).
+template <bool PAIR> constexpr int RUN = PAIR ? 12 : 8;
+constexpr int RUN_ALONE = 8;
 constexpr int EPI_WARPS = 8, HEAD_THREADS = 64 + 32 * EPI_WARPS;
 constexpr int COLS = BN / 2;                                    // columns of a thread: two warps share 32 lanes
 constexpr int ERR_BASE = 64;
@@ -115,7 +121,7 @@ head_logprobs_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
   const int n_tt = (p.R + TILE_ROWS - 1) / TILE_ROWS, n_vt = (p.V + BN - 1) / BN;
   const long n_tiles = (long)n_vt * n_tt;
   const int nkb = (p.K + KS * BK - 1) / (KS * BK);               // stages a tile: a last one that K does not fill multiplies zeros
-  const int runs = nkb * KS <= RUN_ALONE ? 1 : nkb * KS <= 2 * RUN ? 2 : (nkb * KS + RUN - 1) / RUN;
+  const int runs = nkb * KS <= RUN_ALONE ? 1 : nkb * KS <= 2 * RUN<PAIR> ? 2 : (nkb * KS + RUN<PAIR> - 1) / RUN<PAIR>;
   const int per_run = (nkb + runs - 1) / runs;                    // runs of nearly equal length; (runs - 1) * per_run < nkb
   const int drop = g_test_drop_from_stage;
 
