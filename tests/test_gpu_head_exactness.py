@@ -1,4 +1,4 @@
-"""How exact the fused head's sums are, where one logit can be read off: weights of two rows, the first of them zeros, so that the log
+"""How exact the fused head's sums and its cap are, where one logit can be read off: weights of two rows, the first of them zeros, so that the log
 probability of the less likely token is minus the other logit."""
 import pytest
 import torch
@@ -36,3 +36,20 @@ def test_sums_of_positive_products(R, K):
     got, want = less_likely(x, w, 0.0)
     off = float((got - want).norm() / want.norm())
     assert off <= 16 * STEP, off / STEP
+
+
+@pytest.mark.parametrize("R", [40, 300])
+@pytest.mark.parametrize("cap", [30.0, 64.0, 65.0, 100.0, 1000.0, 1e4, 1e30])
+def test_caps_of_any_size(R, cap):
+    """Logits that are exact (one product of a row is not zero).  The capped logit is within 4 steps of a logit's size, or of 64 where the
+    cap is below that (a quotient's error counts with the cap); the log probability adds at most two."""
+    g = torch.Generator(device=DEV).manual_seed(R)
+    x = torch.zeros(R, 64, device=DEV)
+    x[:, 3] = 120.0 * torch.rand(R, generator=g, device=DEV) - 60.0
+    x[0, 3], x[1, 3], x[2, 3], x[3, 3] = 250.0, -250.0, 0.25, 0.0
+    x = x.to(torch.bfloat16)
+    w = torch.zeros(2, 64, dtype=torch.bfloat16, device=DEV)
+    w[1, 3] = 1.0
+    got, want = less_likely(x, w, cap)
+    size = want.abs().clamp(min=64.0 if cap <= 64.0 else 0.6)
+    assert bool(((got - want).abs() <= 6 * STEP * size).all()), float(((got - want).abs() / size).max() / STEP)
