@@ -1496,8 +1496,8 @@ def head_logprobs(x, weight, tokens, out_logprob, *, out_entropy=None, softcap: 
     for t in (x, weight):
         if t.dtype not in (torch.float32, torch.bfloat16) or not t.is_contiguous():
             raise KernelError(f"{what}: x and weight are contiguous float32 or bfloat16 (got {t.dtype})")
-    if not 0.0 <= softcap < float("inf"):
-        raise KernelError(f"{what}: softcap {softcap} is not 0 or a positive number")
+    if not (softcap == 0.0 or 2.0 ** -126 <= softcap <= 2.0 ** 126):       # what twice and one over are in 32 bits too
+        raise KernelError(f"{what}: softcap {softcap} is not 0 or a positive number of 32 bits (2^-126 to 2^126)")
     (R, K), V = x.shape, weight.shape[0]
     if tokens is None or out_logprob is None:
         raise KernelError(f"{what}: tokens and out_logprob are needed")
