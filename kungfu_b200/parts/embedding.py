@@ -89,9 +89,11 @@ class LmHead(Part):
             ops.head_logprobs(h, self.weight, tokens, rows.logprob, out_entropy=rows.entropy, softcap=self.softcap)
             return
         step = max(1, min(n, ops.LOGITS_PIECE_BYTES // (4 * self.vocab)))
+        # from the allocator and back to it: a step buffer that grows would have every captured graph thrown away, and stay
+        piece = torch.empty((step, self.vocab), dtype=torch.float32, device=h.device)
         for a in range(0, n, step):
             b = min(n, a + step)
-            logits = ctx.buf("score_logits", (b - a, self.vocab), torch.float32)
+            logits = piece[:b - a]
             ops.linear(h[a:b], self.weight, logits, softcap=self.softcap)
             ops.token_logprobs(logits, tokens[a:b], rows.logprob[a:b], out_entropy=rows.entropy[a:b], out_rank=rows.rank[a:b],
                                out_top_ids=rows.ids[a:b], out_top_logprobs=rows.top_logprobs[a:b])
