@@ -186,8 +186,7 @@ def cmd_generate(args) -> int:
                         repeat_penalty=args.repeat_penalty)
     if args.logprobs is not None:
         rid = eng.add_request(ids, sampling, max_tokens=args.max_tokens, ignore_eos=args.ignore_eos, seed=args.seed, logprobs=args.logprobs)
-        while not eng.idle:
-            eng.step()
+        eng.run_to_end([rid])
         req = eng.requests[rid]
         print(json.dumps({"prompt": ids, "generated": req.output, "scores": [_score_fields(t) for t in req.scores]}))
         return 0

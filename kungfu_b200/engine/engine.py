@@ -312,6 +312,11 @@ class Engine:
         """Token ids in, generated token ids out, one list per prompt (host lists both ways)."""
         ids = [self.add_request(p, sampling, max_tokens=max_tokens, eos=eos, ignore_eos=ignore_eos, seed=seed + i)
                for i, p in enumerate(prompts)]
+        self.run_to_end(ids)
+        return [list(self.requests[i].output) for i in ids]
+
+    def run_to_end(self, ids: Sequence[Hashable]) -> None:
+        """Step until these requests are finished and nothing is in flight; raises what a kernel has recorded on the device."""
         while any(self.requests[i].status != "finished" for i in ids) or self._inflight is not None:
             before = sum(len(self.requests[i].output) for i in ids)
             ev = self.step()
@@ -319,7 +324,6 @@ class Engine:
                 break
         if self.runner.device.type == "cuda":
             ops.raise_on_device_error(self.runner.device)
-        return [list(self.requests[i].output) for i in ids]
 
     # ---- scoring, forks, beams -----------------------------------------------------------------------------------
     def score(self, prompts: Sequence[Sequence[int]], *, top: int = 0) -> list[list[TokenScore]]:
