@@ -180,21 +180,22 @@ def cmd_generate(args) -> int:
     eng = _engine(args, parallel=max(1, args.beams))
     if args.beams > 1:
         found = eng.beam_search(ids, beams=args.beams, max_tokens=args.max_tokens, ignore_eos=args.ignore_eos)
-        print(json.dumps({"prompt": ids, "beams": [{"generated": b.tokens, "logprob": b.logprob, "finish": b.finish_reason} for b in found]}))
+        def text(b):
+            return b.tokens[:-1] if b.finish_reason == "eos" and not args.emit_ids else b.tokens
+        print(json.dumps({"prompt": ids, "beams": [{"generated": text(b), "logprob": b.logprob, "finish": b.finish_reason} for b in found]}))
         return 0
     sampling = Sampling(temperature=args.temperature, top_k=args.top_k, top_p=args.top_p, min_p=args.min_p,
                         repeat_penalty=args.repeat_penalty)
-    if args.logprobs is not None:
-        rid = eng.add_request(ids, sampling, max_tokens=args.max_tokens, ignore_eos=args.ignore_eos, seed=args.seed, logprobs=args.logprobs)
-        eng.run_to_end([rid])
-        req = eng.requests[rid]
-        print(json.dumps({"prompt": ids, "generated": req.output, "scores": [_score_fields(t) for t in req.scores]}))
-        return 0
-    out = eng.generate([ids], sampling, max_tokens=args.max_tokens, ignore_eos=args.ignore_eos, seed=args.seed)[0]
+    rid = eng.add_request(ids, sampling, max_tokens=args.max_tokens, ignore_eos=args.ignore_eos, seed=args.seed, logprobs=args.logprobs)
+    eng.run_to_end([rid])
+    out, scores = eng.requests[rid].output, eng.requests[rid].scores
     eos = set(getattr(eng.cfg, "eos_token_id", ()) or ())
     if out and out[-1] in eos and not args.ignore_eos and not args.emit_ids:
-        out = out[:-1]
-    print(json.dumps({"prompt": ids, "generated": out}))
+        out, scores = out[:-1], scores[:-1]
+    doc = {"prompt": ids, "generated": out}
+    if args.logprobs is not None:
+        doc["scores"] = [_score_fields(t) for t in scores]
+    print(json.dumps(doc))
     return 0
 
 

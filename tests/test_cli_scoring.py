@@ -1,5 +1,6 @@
 """The commands that report log probabilities, in this process: on the CPU stand-in, and what a device has recorded on the GPU."""
 import json
+from types import SimpleNamespace
 
 import pytest
 import torch
@@ -19,14 +20,15 @@ def folder(tmp_path_factory):
 
 @pytest.fixture
 def program(folder, cpu_ops, monkeypatch, capsys):
-    """A function that runs a command on the CPU stand-in and gives what it prints; `.engines`: the engines it made."""
+    """A function that runs a command on the CPU stand-in and gives what it prints; `.engines`: the engines it made, `.eos`: the ids
+    that end a text."""
     engines = []
 
     def engine(args, parallel=1):
         cfg, model = api.load_model(folder, dtype="float32", device="cpu")
         runner = api.make_runner(cfg, model, dtype="float32", device="cpu", page_size=4, max_tokens=256, max_requests=max(parallel, 2), max_context=64)
         engines.append(Engine(runner=runner, batch=16, parallel=max(parallel, 2)))
-        engines[-1].cfg = cfg
+        engines[-1].cfg = SimpleNamespace(eos_token_id=run.eos)
         return engines[-1]
 
     def run(*args):
@@ -34,7 +36,7 @@ def program(folder, cpu_ops, monkeypatch, capsys):
         return json.loads(capsys.readouterr().out)
 
     monkeypatch.setattr(cli, "_engine", engine)
-    run.engines = engines
+    run.engines, run.eos = engines, ()
     return run
 
 
@@ -57,3 +59,25 @@ def test_a_scored_generation_runs_as_the_plain_one(program, monkeypatch):
     scored = program("generate", "--max-tokens", "6", "--ignore-eos", "--logprobs", "2")
     assert scored["generated"] == plain["generated"] and [s["token"] for s in scored["scores"]] == plain["generated"]
     assert len(ends) == 2
+
+
+def test_the_id_that_ends_a_text_is_taken_off_its_scores_too(program):
+    ids = program("generate", "--max-tokens", "8", "--ignore-eos")["generated"]
+    program.eos = (ids[4],)
+    n = ids.index(ids[4])
+    plain = program("generate", "--max-tokens", "8")
+    scored = program("generate", "--max-tokens", "8", "--logprobs", "0")
+    assert plain["generated"] == scored["generated"] == ids[:n] and [s["token"] for s in scored["scores"]] == ids[:n]
+    whole = program("generate", "--max-tokens", "8", "--logprobs", "0", "--emit-ids")
+    assert whole["generated"] == ids[:n + 1] and [s["token"] for s in whole["scores"]] == ids[:n + 1]
+
+
+def test_the_id_that_ends_a_text_is_taken_off_beams(program):
+    program.eos = tuple(range(0, 512, 5))
+    bare = program("generate", "--max-tokens", "6", "--beams", "4")["beams"]
+    whole = program("generate", "--max-tokens", "6", "--beams", "4", "--emit-ids")["beams"]
+    assert any(b["finish"] == "eos" for b in whole)
+    for a, b in zip(bare, whole):
+        ended = b["finish"] == "eos"
+        assert (b["generated"][-1] in program.eos) == ended and a["logprob"] == b["logprob"]
+        assert a["generated"] == (b["generated"][:-1] if ended else b["generated"])
