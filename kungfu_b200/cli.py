@@ -176,8 +176,15 @@ def cmd_generate(args) -> int:
     from .sampling import Sampling
     if args.ids is None:
         raise SystemExit("error: this build has no tokenizer; give the prompt as --ids '[1, 2, 3]'")
+    if args.beams < 1:
+        raise SystemExit(f"error: --beams {args.beams} is not a number of answers")
+    if args.beams > 1:
+        for name, given in (("--temperature", args.temperature != 0.0), ("--repeat-penalty", args.repeat_penalty != 1.0),
+                            ("--min-p", args.min_p != 0.0), ("--logprobs", args.logprobs is not None)):
+            if given:
+                raise SystemExit(f"error: a beam search draws no tokens and scores none by itself: --beams goes without {name}")
     ids = json.loads(args.ids)
-    eng = _engine(args, parallel=max(1, args.beams))
+    eng = _engine(args, parallel=args.beams)
     if args.beams > 1:
         found = eng.beam_search(ids, beams=args.beams, max_tokens=args.max_tokens, ignore_eos=args.ignore_eos)
         def text(b):
@@ -213,6 +220,10 @@ def cmd_score(args) -> int:
     import torch
     from .engine.step import StepEntry
     ids = json.loads(args.ids)
+    if args.logprobs:
+        for name, given in (("--prefix", args.prefix is not None), ("--ignore-eos", args.ignore_eos)):
+            if given:
+                raise SystemExit(f"error: the ids themselves are scored, nothing is predicted: --logprobs goes without {name}")
     eng = _engine(args)
     if args.logprobs:
         scores = eng.score([ids], top=args.topk)[0]

@@ -81,3 +81,12 @@ def test_the_id_that_ends_a_text_is_taken_off_beams(program):
         ended = b["finish"] == "eos"
         assert (b["generated"][-1] in program.eos) == ended and a["logprob"] == b["logprob"]
         assert a["generated"] == (b["generated"][:-1] if ended else b["generated"])
+
+
+@pytest.mark.parametrize("args", [("generate", "--beams", "0"), ("generate", "--beams", "-3")] + [("generate", "--beams", "2", *more) for more in (
+    ("--temperature", "0.7"), ("--repeat-penalty", "1.2"), ("--min-p", "0.1"), ("--logprobs", "0"))] + [
+        ("score", "--logprobs", "--prefix", "3"), ("score", "--logprobs", "--ignore-eos")])
+def test_options_that_would_have_no_effect_are_refused(program, args):
+    with pytest.raises(SystemExit, match="error: .*--"):
+        program(*args)
+    assert not program.engines
