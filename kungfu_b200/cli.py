@@ -228,8 +228,9 @@ def cmd_score(args) -> int:
     if args.logprobs:
         scores = eng.score([ids], top=args.topk)[0]
         total = sum(t.logprob for t in scores)
-        print(json.dumps({"ids": ids, "logprob": total, "perplexity": math.exp(-total / max(len(scores), 1)),
-                          "scores": [_score_fields(t) for t in scores]}))
+        mean = -total / max(len(scores), 1)
+        perplexity = math.inf if mean > 709.0 else math.exp(mean)     # (exp(710) is more than a double holds)
+        print(json.dumps({"ids": ids, "logprob": total, "perplexity": perplexity, "scores": [_score_fields(t) for t in scores]}))
         return 0
     runner = eng.runner
     prefix = len(ids) if args.prefix is None else max(1, min(args.prefix, len(ids)))

@@ -8,6 +8,7 @@ import torch
 import helpers
 from kungfu_b200 import api, cli, ops
 from kungfu_b200.engine.engine import Engine
+from kungfu_b200.sampling import TokenScore
 
 CFG = helpers.TINY_A
 IDS = helpers.random_tokens(9, 512, 2)
@@ -90,3 +91,11 @@ def test_options_that_would_have_no_effect_are_refused(program, args):
     with pytest.raises(SystemExit, match="error: .*--"):
         program(*args)
     assert not program.engines
+
+
+@pytest.mark.parametrize("logprob,perplexity", [(-2.0, 7.38905609893065), (-700.0, 1.0142320547350045e304), (-5000.0, float("inf")),
+                                                (float("-inf"), float("inf")), (float("nan"), float("nan"))])
+def test_the_perplexity_of_any_text(program, monkeypatch, logprob, perplexity):
+    monkeypatch.setattr(Engine, "score", lambda self, prompts, top=0: [[TokenScore(t, logprob, 1.0) for t in p[1:]] for p in prompts])
+    doc = program("score", "--logprobs")
+    assert doc["perplexity"] == pytest.approx(perplexity, nan_ok=True)
