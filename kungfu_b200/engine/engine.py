@@ -19,7 +19,7 @@ from .. import events as _events
 from .. import ops
 from ..cache.manager import CacheError, OutOfPages
 from ..sampling.sampler import STATE_WORDS, Sampling, pack_state
-from ..sampling.scores import ScoreRows, TokenScore, check_alternatives
+from ..sampling.scores import MAX_ALTERNATIVES, ScoreRows, TokenScore, check_alternatives
 from .scheduler import Request, Scheduler
 from .step import Runner, StepEntry
 
@@ -432,9 +432,9 @@ class Engine:
     def beam_search(self, prompt: Sequence[int], *, beams: int = 4, max_tokens: int = 64, eos: Sequence[int] | None = None,
                     ignore_eos: bool = False, length_penalty: float = 0.0) -> list[Beam]:
         """The `beams` best answers found by a search that keeps that many open ones, best first.  An answer's value is the sum of its
-        tokens' log probabilities over length ** length_penalty.  Every step asks each open answer for its 2 * beams best next tokens;
-        the cache of an answer that goes on in several ways is forked, that of a dropped one freed.  At most 32 beams, and no more than
-        the cache has free state slots."""
+        tokens' log probabilities over length ** length_penalty.  Every step asks each open answer for its 2 * beams best next tokens, or
+        for as many as leave `beams` of them beside every id of `eos`, but no more than 64; the cache of an answer that goes on in several ways
+        is forked, that of a dropped one freed.  At most 32 beams, and no more than the cache has free state slots."""
         prompt = [int(t) for t in prompt]
         cache, vocab = self.runner.cache, self.runner.vocab
         if not prompt or any(not (0 <= t < vocab) for t in prompt):
@@ -449,7 +449,7 @@ class Engine:
         if eos is None:
             eos = tuple(getattr(self.cfg, "eos_token_id", ()) or ()) if self.cfg is not None else ()
         eos = set() if ignore_eos else set(eos)
-        top = min(2 * beams, vocab)
+        top = min(max(2 * beams, beams + len(eos)), MAX_ALTERNATIVES, vocab)
 
         def value(logprob, n):
             return logprob / n ** length_penalty
