@@ -491,11 +491,6 @@ int launch_type(const void* logits, long ld, int R, int V, const int* tokens, fl
 
 }  // namespace
 
-#ifdef KF_TUNING
-static int g_slices = 0;
-KF_API void kf_token_logprobs_slices(int n) { g_slices = n; }
-#endif
-
 // logits [R, V] of element type dt (KF_F32, KF_BF16), rows ld elements apart; tokens [R] (null: only entropy and alternatives;
 // a negative one: the row's outputs stay as they are; one >= V, or one whose logit is NaN: NaN and rank -1); every output may be null; top <= 64, <= V.
 KF_API int kf_token_logprobs(const void* logits, int dt, long ld, int R, int V, const int* tokens, float* logprob, float* entropy,
@@ -503,15 +498,12 @@ KF_API int kf_token_logprobs(const void* logits, int dt, long ld, int R, int V, 
   if (R <= 0) return KF_OK;
   if (V <= 0 || V > 0x7fffff00 || R > (1 << 27) || top < 0 || top > TOP_MAX || top > V || (!tokens && (logprob || rank))) return KF_ERR_SIZE;
   if (((uintptr_t)logits & (dt == KF_F32 ? 3 : 1)) != 0) return KF_ERR_ALIGN;
-  // A row is cut while its slices still fit the device at once (two blocks an SM) and none falls below a chunk.  32-bit logits, L2
+  // A row is cut while its slices still fit the device at once (two blocks an SM) and each is more than half a chunk.  32-bit logits, L2
   // flushed, slices 1 / 2 / 4 / 8 / 16: 64 x 256,000 with 20 alternatives 49 / 35 / 31 / 39 / 56 us, 8 x 256,000 47 / 32 / 23 / 18 / 18,
   // 512 x 256,000 132 / 139 / 174 / 228 / 339, 301 x 32,003 28 / 35 / 43 / 74 / 142.
   const int chunks = kf_ceil_div(V, CHUNK);
   int slices = 1;
   while (slices < MAX_SLICES && slices < chunks && (long)R * slices <= kf_sm_count()) slices *= 2;
-#ifdef KF_TUNING
-  if (g_slices > 0) slices = g_slices;
-#endif
   // Rows of a few chunks that need more than two blocks an SM: a block's start and end are most of its time, and a third block hides more of
   // them than loads ahead do.  2,048 x 32,000 with 20 alternatives 100 us ahead, 92 not, without alternatives 57 and 54; 301 x 32,003 with
   // 64 alternatives 38 and 35; 512 x 256,000 89 and 115.
