@@ -85,8 +85,8 @@ __device__ __forceinline__ float min_nan(float a, float b) {
   return r;
 }
 // 1 / d for d in [1, 2^41], two at a time on the FMA units (the hardware's reciprocal shares its unit with the exponential, which bounds
-// the epilogue): a first guess from the exponent's and fraction's bits (of all constants to subtract them from, the one whose
-// largest error is least, 5.1 %), and three Newton-Raphson steps r (2 - d r), each of which squares the error.
+// the epilogue): a first guess from the exponent's and fraction's bits (a constant less these; its largest error is 5.05 %, and neighbouring
+// constants differ in the fifth digit), and three Newton-Raphson steps r (2 - d r), each of which squares the error.
 __device__ __forceinline__ u64 reciprocal2(u64 d) {
   const float2 f = kf_row::unpack2(d);
   u64 r = kf_row::pack2(__int_as_float(0x7ef31200 - __float_as_int(f.x)), __int_as_float(0x7ef31200 - __float_as_int(f.y)));
@@ -323,7 +323,7 @@ head_logprobs_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
       if (!ok || idle) continue;
       if (p.cap > 0.f) {
         // cap tanh(v / cap) = cap - 2 cap / (exp(2 v / cap) + 1): within 2e-7 of the cap.  From 2^40 on the quotient is nothing.  Up to
-        // WIDE_CAP that is less than the sums' own errors; beyond it small logits would lose what the cap is larger than they.
+        // WIDE_CAP that is 1.3e-5 of a logit at most; a larger cap would take the digits of small logits.
         const u64 in = kf_row::pack2(2.f * kf_row::LOG2E / p.cap, 2.f * kf_row::LOG2E / p.cap), one = kf_row::pack2(1.f, 1.f);
         const u64 twice = kf_row::pack2(-2.f * p.cap, -2.f * p.cap), cap2 = kf_row::pack2(p.cap, p.cap);
         auto quotient_form = [&](float a, float b) {
