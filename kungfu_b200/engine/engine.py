@@ -329,7 +329,8 @@ class Engine:
     def score(self, prompts: Sequence[Sequence[int]], *, top: int = 0) -> list[list[TokenScore]]:
         """For every prompt, one `TokenScore` for each of its tokens but the first: how likely it was after those before it, and how
         many alternatives `top` asks for (0 to 64; without any, the logits are never stored and no ranks come back).  Prompts run
-        in portions of up to `batch` tokens, several prompts in a step, beside whatever the cache holds of running requests."""
+        in portions of up to `batch` tokens, several prompts in a step, beside whatever the cache holds of running requests.  Raises
+        CacheError or OutOfPages if those leave no state slot or no pages."""
         prompts = [[int(t) for t in p] for p in prompts]
         top = check_alternatives(top, self.runner.vocab)
         cache, vocab = self.runner.cache, self.runner.vocab
@@ -365,6 +366,8 @@ class Engine:
                     targets.append(prompts[i][at + 1:at + n + 1])
                     room -= n
                 if not entries:
+                    if not fed and cache.n_live >= cache.max_requests:
+                        raise CacheError(f"no state slot is free for a prompt to score ({cache.n_live} live requests)")
                     raise OutOfPages("no page is free for the prompts to score")
                 rows = self.runner.score(entries, targets, top)
                 flat = [t for ts in targets for t in ts]
