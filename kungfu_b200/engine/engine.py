@@ -403,11 +403,12 @@ class Engine:
         return all(a <= b for a, b in zip(need, cache.free_pages()))
 
     def fork(self, request_id: Hashable, *, new_id: Hashable | None = None, seed: int | None = None, sampling: Sampling | None = None,
-             max_tokens: int | None = None, logprobs: int | None = None) -> Hashable:
+             max_tokens: int | None = None, logprobs: int | str | None = "inherit") -> Hashable:
         """Another request that goes on from where `request_id` stands (which must be producing tokens): the same prompt, the same output so
         far, the same cached context, of which only the last page and the recurrent states are copied.  It draws by its own
-        generator (`seed`, default one more than the parent's), and by other rules, lengths or scores if given.  Raises OutOfPages or CacheError if the cache
-        has no page or state slot for it."""
+        generator (`seed`, default one more than the parent's: forks of one parent that are to differ need seeds of their own), and by other
+        rules and lengths if given.  `logprobs`: as of `add_request` (None: no scores); by default the parent's.  Raises OutOfPages or
+        CacheError if the cache has no page or state slot for it."""
         self._held = self.flush()
         parent = self.requests[request_id]
         if not parent.decoding:
@@ -415,6 +416,8 @@ class Engine:
         limit = parent.max_tokens if max_tokens is None else int(max_tokens)
         if limit <= len(parent.output):
             raise ValueError(f"max_tokens {limit} is not above the {len(parent.output)} tokens already produced")
+        if logprobs == "inherit":
+            logprobs = parent.logprobs
         if logprobs is not None:
             logprobs = check_alternatives(logprobs, self.runner.vocab)
         if new_id is None:
@@ -424,8 +427,9 @@ class Engine:
             raise ValueError(f"request id {new_id!r} is in use")
         req = Request(new_id, list(parent.prompt), sampling or parent.sampling, max_tokens=limit, eos=parent.eos,
                       ignore_eos=parent.ignore_eos, seed=parent.seed + 1 if seed is None else seed,
-                      logprobs=parent.logprobs if logprobs is None else logprobs)
-        req.output, req.n_cached, req.scores = list(parent.output), parent.n_cached, list(parent.scores)
+                      logprobs=logprobs)
+        req.output, req.n_cached = list(parent.output), parent.n_cached
+        req.scores = [] if logprobs is None else list(parent.scores)
         self.runner.cache.fork(request_id, new_id)
         self.scheduler.adopt(req)
         self.requests[new_id] = req

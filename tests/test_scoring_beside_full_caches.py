@@ -32,3 +32,16 @@ def test_a_score_without_a_state_slot_says_so(engine):
     while not engine.idle:
         engine.step()
     assert len(engine.score([[1, 2, 3]])[0]) == 2 and all(len(engine.requests[i].output) == 5 for i in ids)
+
+
+def test_a_fork_without_its_parents_scores(engine):
+    a = engine.add_request([5, 2, 3], Sampling(temperature=0.0), max_tokens=7, ignore_eos=True, logprobs=2)
+    while len(engine.requests[a].output) < 3:
+        engine.step()
+    b, c = engine.fork(a, logprobs=None), engine.fork(a)
+    with pytest.raises(ValueError):
+        engine.fork(a, logprobs=65)
+    while not engine.idle:
+        engine.step()
+    assert engine.requests[b].scores == [] and engine.requests[b].logprobs is None
+    assert [len(engine.requests[i].scores) for i in (a, c)] == [7, 7] and engine.requests[a].output == engine.requests[b].output
