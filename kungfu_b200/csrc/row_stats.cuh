@@ -47,13 +47,13 @@ __device__ __forceinline__ u64 fma2(u64 a, u64 b, u64 c) {
 }
 
 // Running maximum (of what is a number), sum of exponentials and sum of d exp(d), and how a second set joins the first.  A NaN
-// among the logits is a NaN in s.  A maximum that lay further than 200 below counts as 200: exp(-200) is 0 in 32 bits, and so is its product with
-// what is finite (the lowest number of all, a common mask, would make d s infinite and u NaN).
+// among the logits is a NaN in s.  A maximum so far below the new one that its terms are 0 beside it leaves nothing: d s may be infinite then (the
+// lowest number of all is a common mask), and times 0 it would be NaN.
 struct Stats { float m, s, u; };
 __device__ __forceinline__ void move_to(Stats& a, float m) {
   if (m != a.m) {
-    const float d = fmaxf(a.m - m, -200.f), f = exp2_fast(d * LOG2E);
-    a.u = a.s == 0.f ? 0.f : f * (a.u + d * a.s);
+    const float d = a.m - m, f = exp2_fast(d * LOG2E);
+    a.u = f == 0.f ? 0.f : f * (a.u + d * a.s);
     a.s *= f;
     a.m = m;
   }
