@@ -16,8 +16,9 @@
 // column must exceed to join them.  The first chunk is cut by a bound that at least k of its columns reach (`warp_bound`) and
 // leaves the exact k-th value as tau.  From then on a column costs one comparison (of the thread's maximum), and a random row
 // brings k * 8,192 / (columns seen) keys a chunk; a list grown long is pruned to its k best, which raises tau.
-// What bounds it: memory for long rows without alternatives (512 x 256,000 in 89 us, 5.9 TB/s); with them the first chunk's bound and
-// ranking and the row's last ranking, which its loads do not cover (512 rows with 20 alternatives 131 us, 64 rows 32, one row 16).
+// What bounds it: memory for long 32-bit rows without alternatives (512 x 256,000 in 89 to 92 us, 5.7 to 5.9 TB/s; bfloat16 78 us, the arithmetic
+// of a column); with them the first chunk's bound and ranking and the row's last ranking, which its loads do not cover (L2 flushed before:
+// 512 rows with 20 alternatives 131 us, 64 rows 31 to 33, one row 14 to 16).
 #include "row_stats.cuh"
 
 namespace {
